@@ -159,8 +159,8 @@ def prepare(case, seed):
                 buffers[key] = torch.empty(shape, dtype=dtype, device=DEV)
             return buffers[key]
 
-        state = {"op": "attention", "heads": (H, G, hd), "q": q, "pages": pages, "page_table": table.to(DEV), "first": first, "count": count,
-                 "starts": starts, "q_start": torch.tensor(starts, dtype=torch.int32, device=DEV),
+        state = {"op": "attention", "heads": (H, G, hd), "q": q, "pages": pages, "page_table": table.to(DEV),
+                 "q_start": torch.tensor(starts, dtype=torch.int32, device=DEV),
                  "kv_len": torch.tensor([f + n for f, n in zip(first, count)], dtype=torch.int32, device=DEV),
                  "shared_pages": len(shared), "max_new": max(count), "out": torch.empty_like(q), "scratch": scratch}
     elif case["op"] == "tables":
@@ -187,15 +187,12 @@ def prepare(case, seed):
         random.Random(seed).shuffle(ids)
         storage = torch.randn(case["layers"], n + 4, 2, G, PAGE, hd, generator=gen, device=DEV, dtype=torch.float32).to(torch.bfloat16)
         state = {"op": "fork", "storage": storage, "sources": [ids[0]] * n, "targets": ids[1:n + 1]}
-    if own:
-        from llmplayer_b200.kernels import ops
-        state["ops"] = ops
     return state
 
 
 # ------------------------------------------------------------------------------------------------ the calls
 def _run_own(state):
-    ops = state["ops"]
+    from llmplayer_b200.kernels import ops
     op = state["op"]
     if op == "logprobs":
         ops.token_logprobs(state["logits"], state["targets"], state["logprob"], state["entropy"], state["rank"],
@@ -216,58 +213,61 @@ def _run_own(state):
 
 
 def _plain_logprobs(logits, targets, top):
-    """Rows a few hundred at a time: exponentials in 32 bits, sums and logarithms in 64 (the probability of a token that is
-    nearly certain differs from one by less than 32 bits show)."""
-    outs = [[] for _ in range(5 if top else 3)]
-    for a in range(0, logits.shape[0], 256):
-        x = logits[a:a + 256].float()
-        t = targets[a:a + 256].long()[:, None]
-        m = x.amax(dim=1, keepdim=True)
-        e = torch.exp(x - m)
-        s = e.sum(dim=1, keepdim=True, dtype=torch.float64)
-        log_s = torch.log(s)
-        # a token without a probability adds nothing to the entropy
-        mean = torch.where(e > 0, e * (x - m), torch.zeros_like(x)).sum(dim=1, keepdim=True, dtype=torch.float64) / s
-        at = x.gather(1, t)
-        index = torch.arange(x.shape[1], device=x.device)[None, :]
-        rank = ((x > at) | ((x == at) & (index < t))).sum(dim=1)
-        outs[0].append(((at - m).double() - log_s).float()[:, 0])
-        outs[1].append((log_s - mean).float()[:, 0])
-        outs[2].append(rank.to(torch.int32))
-        if top:
-            values, ids = torch.sort(x, dim=1, descending=True, stable=True)         # equal ones: the lowest index first
-            outs[3].append(ids[:, :top].to(torch.int32))
-            outs[4].append(((values[:, :top] - m).double() - log_s).float())
-    return [torch.cat(o) for o in outs]
+    """Exponentials in 32 bits, their sums and logarithms in 64 (the probability of a token that is nearly certain differs from
+    one by less than 32 bits show)."""
+    x, t = logits.float(), targets.long()[:, None]
+    m = x.amax(dim=1, keepdim=True)
+    e = torch.exp(x - m)
+    s = e.sum(dim=1, keepdim=True, dtype=torch.float64)
+    log_s = torch.log(s)
+    # a token without a probability adds nothing to the entropy
+    mean = torch.where(e > 0, e * (x - m), torch.zeros_like(x)).sum(dim=1, keepdim=True, dtype=torch.float64) / s
+    at = x.gather(1, t)
+    index = torch.arange(x.shape[1], device=x.device)[None, :]
+    rank = ((x > at) | ((x == at) & (index < t))).sum(dim=1)
+    out = [((at - m).double() - log_s).float()[:, 0], (log_s - mean).float()[:, 0], rank.to(torch.int32)]
+    if top:
+        values, ids = torch.sort(x, dim=1, descending=True, stable=True)             # equal ones: the lowest index first
+        out += [ids[:, :top].to(torch.int32), ((values[:, :top] - m).double() - log_s).float()]
+    return out
+
+
+def _softmax_parts(scores, values):
+    """The weighted sum of the values with the weights' sum and the maximum that they are taken against."""
+    m = scores.amax(dim=-1, keepdim=True)
+    weights = scores.sub_(m).exp_()
+    return weights @ values, weights.sum(dim=-1, keepdim=True), m
 
 
 def _plain_attention(state):
     H, G, hd = state["heads"]
-    R = H // G
-    scale = hd ** -0.5
-    q, pages, P = state["q"].float(), state["pages"], state["shared_pages"]
-    table = state["page_table"].long()
-
-    def dense(ids):                                        # [G, positions, hd] of the pages named
-        kv = pages[ids].float()
-        return (kv[:, 0].permute(1, 0, 2, 3).reshape(G, -1, hd), kv[:, 1].permute(1, 0, 2, 3).reshape(G, -1, hd))
-
-    k0, v0 = dense(table[0, :P])
-    outs = []
-    for b, (first, n) in enumerate(zip(state["first"], state["count"])):
-        a = state["starts"][b]
-        rows = q[a:a + n].view(n, G, R, hd).permute(1, 2, 0, 3).reshape(G, R * n, hd)
-        last = first + n
-        k1, v1 = dense(table[b, P:-(-last // PAGE)])
-        scores = torch.cat([rows @ k0.transpose(1, 2), rows @ k1.transpose(1, 2)], dim=2) * scale
-        position = torch.arange(first, last, device=q.device).repeat(R)[None, :, None]
-        key = torch.arange(scores.shape[2], device=q.device)[None, None, :]
-        scores = torch.where(key <= position, scores, torch.full_like(scores, float("-inf")))
-        weights = torch.exp(scores - scores.amax(dim=2, keepdim=True))
-        total = weights.sum(dim=2, keepdim=True)
-        o = (weights[:, :, :P * PAGE] @ v0 + weights[:, :, P * PAGE:] @ v1) / total
-        outs.append(o.view(G, R, n, hd).permute(2, 0, 1, 3).reshape(n, H * hd))
-    return torch.cat(outs).to(torch.bfloat16)
+    R, P = H // G, state["shared_pages"]
+    pages, table, starts, kv_len = state["pages"], state["page_table"].long(), state["q_start"].long(), state["kv_len"].long()
+    T, B, n = state["q"].shape[0], kv_len.numel(), state["max_new"]
+    q = state["q"].float().view(T, G, R, hd) * hd ** -0.5
+    # over the shared pages: all tokens' queries at once, [G, T R, positions]; every token sees all of them
+    kv = pages[table[0, :P]].float()
+    k0, v0 = (kv[:, which].permute(1, 0, 2, 3).reshape(G, P * PAGE, hd) for which in (0, 1))
+    o0, l0, m0 = _softmax_parts(q.permute(1, 0, 2, 3).reshape(G, T * R, hd) @ k0.transpose(1, 2), v0)
+    o0, l0, m0 = (x.view(G, T, R, -1).permute(1, 0, 2, 3) for x in (o0, l0, m0))
+    # over each sequence's own pages: the tokens in a batch that is filled up to the longest run, [B, G, n R, positions]
+    j = torch.arange(n, device=q.device)[None, :]
+    count = (starts[1:] - starts[:-1])[:, None]
+    token = (starts[:-1, None] + j).clamp(max=T - 1)
+    position = (kv_len[:, None] - count + j)[:, None, :, None, None]                   # [B, 1, n, 1, 1]
+    kv = pages[table[:, P:]].float()                                                   # [B, W, 2, G, PAGE, hd]
+    k1, v1 = (kv[:, :, which].permute(0, 2, 1, 3, 4).reshape(B, G, -1, hd) for which in (0, 1))
+    scores = q[token].permute(0, 2, 1, 3, 4).reshape(B, G, n * R, hd) @ k1.transpose(2, 3)
+    key = P * PAGE + torch.arange(k1.shape[2], device=q.device)
+    hidden = (key > position).expand(B, G, n, R, -1).reshape(scores.shape)
+    o1, l1, m1 = _softmax_parts(scores.masked_fill_(hidden, float("-inf")), v1)
+    sequence = torch.repeat_interleave(torch.arange(B, device=q.device), count[:, 0], output_size=T)
+    place = torch.arange(T, device=q.device) - starts[sequence]
+    o1, l1, m1 = (x.view(B, G, n, R, -1).permute(0, 2, 1, 3, 4)[sequence, place] for x in (o1, l1, m1))
+    # the two parts against their common maximum
+    m = torch.maximum(m0, m1)
+    f0, f1 = torch.exp(m0 - m), torch.exp(m1 - m)
+    return ((o0 * f0 + o1 * f1) / (l0 * f0 + l1 * f1)).reshape(T, H * hd).to(torch.bfloat16)
 
 
 def _plain_tables(state):
