@@ -41,6 +41,8 @@ LIBRARIES: Dict[str, str] = {
     "chunked_recurrence": "chunked_recurrence.cu",
     "recurrent_step": "recurrent_step.cu",
     "stream_bundle": "stream_bundle.cu",
+    "scoring": "scoring.cu",
+    "shared_prefix": "shared_prefix.cu",
 }
 HEADERS = ("common.cuh", "attention_noalloc.h", "tcgen05_utils.cuh", "attention_decode.cuh", "bf16_parts.cuh")
 

@@ -138,6 +138,16 @@ _SIGNATURES = {
         "lp_argmax": [_P, ctypes.c_longlong, _I, _I, _P, _P, _P],
         "lp_sample_fetch": [_P, _P, _I, _I, _I, _I, _P],
     },
+    "scoring": {
+        "lp_token_logprobs_most_top": [],
+        "lp_token_logprobs": [_P, _I, ctypes.c_longlong, _P, _P, _P, _P, _P, _P, _I, _I, _I, _P],
+    },
+    "shared_prefix": {
+        "lp_step_tables": [_P, _P, _P, _I, _P, _I, _P, _P, _P, _P, _I, _P, _I, _I, _I, _P],
+        "lp_copy_pages_most": [],
+        "lp_copy_pages": [_P, _I, ctypes.c_longlong, ctypes.c_longlong, _P, _P, _I, _P],
+        "lp_attention_shared": [_P, _P, _P, _P, _I, _P, _P, _I, _I, _I, _I, _I, _I, _F, _P],
+    },
 }
 
 _libs: Dict[str, ctypes.CDLL] = {}
@@ -404,6 +414,14 @@ def _want(t: torch.Tensor, what: str, dtype=None, ndim: Optional[int] = None) ->
 
 def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
     return None if t is None else t.data_ptr()
+
+
+def _on_current_device(what: str, *tensors: Optional[torch.Tensor]) -> None:
+    """All on the device whose stream the launch goes to."""
+    device = torch.cuda.current_device()
+    for t in tensors:
+        if t is not None and t.device.index != device:
+            raise KernelError(f"{what}: a tensor on {t.device}, the current device is cuda:{device}")
 
 
 # --------------------------------------------------------------------------- embedding
@@ -1247,6 +1265,117 @@ def attention(ctx, q: torch.Tensor, out: torch.Tensor, pages: torch.Tensor, page
                            num_kv_heads=num_kv_heads, head_dim=head_dim, scale=scale, window=window, softcap=softcap,
                            sinks=sinks, keep_first=keep_first, chunk=chunk, distance=distance, gate=gate,
                            scratch=ctx.buffer if ctx.max_new <= PLAIN_PARTS_TOKENS else None)
+
+
+def attention_shared_serves(num_heads: int, num_kv_heads: int, head_dim: int, page_size: int = 64) -> bool:
+    """Whether :func:`attention_shared` is built for these heads."""
+    return (head_dim in (64, 128) and page_size == 64 and num_kv_heads > 0 and num_heads % num_kv_heads == 0
+            and num_heads // num_kv_heads <= 128)
+
+
+def attention_shared(q: torch.Tensor, out: torch.Tensor, pages: torch.Tensor, page_table: torch.Tensor, q_start: torch.Tensor,
+                     kv_len: torch.Tensor, scratch, *, shared_pages: int, max_new: int, num_heads: int, num_kv_heads: int,
+                     head_dim: int, scale: float) -> torch.Tensor:
+    """Attention of a batch whose sequences share their first ``shared_pages`` pages: the first so many columns of
+    ``page_table`` [B, W] are the same in every row. The new tokens of all sequences attend over those pages together, so that
+    a page is read once for the whole batch, and each sequence's tokens over its own pages behind them.
+
+    ``q``, ``out``: bfloat16 [T, H * hd], the new tokens of the sequences one behind the other; ``q_start`` int32 [B + 1]: where
+    each sequence's begin (a sequence may have none); ``kv_len`` int32 [B]: lengths with the new tokens; ``max_new``: no sequence has
+    more new tokens. A token sees its sequence's keys up to its own position. Rows of ``q`` behind the last sequence are not
+    read, and those of ``out`` stay as they are. ``scratch(name, shape, dtype)`` supplies buffers for partial results."""
+    what = "attention_shared"
+    _check_attention(q, out, pages, page_table, num_heads, num_kv_heads, head_dim, what)
+    _want(q_start, f"{what} q_start", torch.int32, 1)
+    _want(kv_len, f"{what} kv_len", torch.int32, 1)
+    _on_current_device(what, q, out, pages, page_table, q_start, kv_len)
+    B, T = kv_len.numel(), q.shape[0]
+    if B == 0 or q_start.numel() != B + 1 or page_table.shape[0] != B:
+        raise KernelError(f"{what}: {B} sequences, {q_start.numel()} offsets, table {tuple(page_table.shape)}")
+    if not attention_shared_serves(num_heads, num_kv_heads, head_dim, pages.shape[3]):
+        raise KernelError(f"{what}: {num_heads} heads on {num_kv_heads} of {head_dim} over pages of {pages.shape[3]} are not served "
+                          f"(heads of 64 or 128, at most 128 per key head, pages of 64)")
+    if not 0 <= int(shared_pages) <= page_table.shape[1]:
+        raise KernelError(f"{what}: {shared_pages} shared pages in tables of {page_table.shape[1]}")
+    if int(max_new) < 1:
+        raise KernelError(f"{what}: at most {max_new} new tokens per sequence")
+    if T == 0:
+        return out
+    lib = library("shared_prefix")
+    _check(lib, lib.lp_attention_shared(q.data_ptr(), out.data_ptr(), pages.data_ptr(), page_table.data_ptr(), page_table.shape[1],
+                                        q_start.data_ptr(), kv_len.data_ptr(), B, T, num_heads, num_kv_heads, head_dim, int(shared_pages),
+                                        float(scale), _stream()))
+    return out
+
+
+# --------------------------------------------------------------------------- a step's tables, copies of pages
+def step_tables(first: torch.Tensor, count: torch.Tensor, shared: torch.Tensor, own: torch.Tensor, q_start: Optional[torch.Tensor],
+                kv_len: Optional[torch.Tensor], positions: Optional[torch.Tensor], seq_ids: Optional[torch.Tensor],
+                page_table: torch.Tensor, *, page_size: int = 64) -> None:
+    """The tables of a step from its sequences' lengths, all int32: sequence b holds ``first[b]`` positions and brings
+    ``count[b]`` new tokens; its blocks of ``page_size`` positions lie in the pages ``shared`` as far as those reach, and behind
+    them in pages of its own, which ``own`` lists sequence after sequence.
+
+    Fills ``page_table`` [B, W] (zero behind a sequence's last block) and, unless they are None (all four), ``q_start`` [B + 1],
+    ``kv_len`` [B] = first + count, and for each new token ``positions`` [T] and the sequence it belongs to, ``seq_ids`` [T].
+    Entries of the latter two behind the last sequence's tokens stay as they are. Nothing is written beyond the
+    tensors' sizes and nothing read beyond ``own``, whatever the lengths say."""
+    what = "step_tables"
+    for t, name in ((first, "first"), (count, "count"), (shared, "shared"), (own, "own")):
+        _want(t, f"{what} {name}", torch.int32, 1)
+    _want(page_table, f"{what} page_table", torch.int32, 2)
+    B = first.numel()
+    if B == 0 or count.numel() != B or page_table.shape[0] != B or page_table.shape[1] == 0:
+        raise KernelError(f"{what}: {B} sequences, {count.numel()} counts, table {tuple(page_table.shape)}")
+    if int(page_size) < 1:
+        raise KernelError(f"{what}: pages of {page_size} positions")
+    rest = (q_start, kv_len, positions, seq_ids)
+    if any(t is None for t in rest) != all(t is None for t in rest):
+        raise KernelError(f"{what}: q_start, kv_len, positions and seq_ids go together")
+    tokens = 0
+    if q_start is not None:
+        for t, name in zip(rest, ("q_start", "kv_len", "positions", "seq_ids")):
+            _want(t, f"{what} {name}", torch.int32, 1)
+        tokens = positions.numel()
+        if q_start.numel() != B + 1 or kv_len.numel() != B or seq_ids.numel() != tokens:
+            raise KernelError(f"{what}: {B} sequences, {q_start.numel()} offsets, {kv_len.numel()} lengths, {tokens} positions of "
+                              f"{seq_ids.numel()} tokens")
+    _on_current_device(what, first, count, shared, own, page_table, *rest)
+    lib = library("shared_prefix")
+    _check(lib, lib.lp_step_tables(first.data_ptr(), count.data_ptr(), shared.data_ptr(), shared.numel(), own.data_ptr(), own.numel(),
+                                   _ptr(q_start), _ptr(kv_len), _ptr(positions), _ptr(seq_ids), tokens, page_table.data_ptr(),
+                                   page_table.shape[1], B, int(page_size), _stream()))
+
+
+def copy_pages(storage: torch.Tensor, sources, targets) -> None:
+    """Copy pages of a cache group's ``storage`` [runs, num_pages, ...] in every run: page ``sources[i]`` to page ``targets[i]``
+    (numbers on the host). A page may be copied to several others; no page is a target twice or a target and a source."""
+    what = "copy_pages"
+    sources, targets = [int(p) for p in sources], [int(p) for p in targets]
+    if len(sources) != len(targets):
+        raise KernelError(f"{what}: {len(sources)} sources and {len(targets)} targets")
+    if not isinstance(storage, torch.Tensor) or storage.dim() < 3:
+        raise KernelError(f"{what}: expected a storage tensor [runs, pages, ...]")
+    num_pages = storage.shape[1]
+    for p in sources + targets:
+        if not 0 <= p < num_pages:
+            raise KernelError(f"{what}: page {p} of {num_pages}")
+    if len(set(targets)) != len(targets) or not set(targets).isdisjoint(sources):
+        raise KernelError(f"{what}: a page is a target twice, or a target and a source")
+    _want(storage, f"{what} storage")
+    _on_current_device(what, storage)
+    page_bytes = storage[0, 0].numel() * storage.element_size() if storage.numel() else 0
+    if not targets or page_bytes == 0:
+        return
+    if page_bytes % 16 or storage.data_ptr() % 16:
+        raise KernelError(f"{what}: pages of {page_bytes} bytes at {storage.data_ptr():#x}: they must be whole vectors of 16 bytes")
+    lib = library("shared_prefix")
+    most = lib.lp_copy_pages_most()
+    for a in range(0, len(targets), most):
+        n = min(most, len(targets) - a)
+        pairs = ctypes.c_int * n
+        _check(lib, lib.lp_copy_pages(storage.data_ptr(), storage.shape[0], num_pages, page_bytes, pairs(*sources[a:a + n]),
+                                      pairs(*targets[a:a + n]), n, _stream()))
 
 
 # --------------------------------------------------------------------------- latent attention
@@ -2530,3 +2659,49 @@ def argmax(logits: torch.Tensor, scratch: torch.Tensor, out_token: torch.Tensor)
         raise KernelError(f"argmax: {B} rows, {out_token.numel()} outputs, scratch of {scratch.numel()}")
     lib = library("sampling")
     _check(lib, lib.lp_argmax(logits.data_ptr(), V, V, B, scratch.data_ptr(), out_token.data_ptr(), _stream()))
+
+
+# --------------------------------------------------------------------------- log probabilities
+TOP_LOGPROBS_MOST = 32        # the longest list of most likely tokens
+
+
+def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, logprob: torch.Tensor, entropy: torch.Tensor, rank: torch.Tensor, *,
+                   top_ids: Optional[torch.Tensor] = None, top_logprobs: Optional[torch.Tensor] = None) -> None:
+    """Per row of ``logits`` (float32 or bfloat16 [R, V]; rows may lie apart): the natural logarithm of the softmax's probability of
+    token ``targets[r]`` (int32) in ``logprob``, the distribution's ``entropy`` in nats (both float32 [R]), and the target's ``rank``
+    (int32 [R]): its place, from 0, in the order of falling logits, equal ones by rising token. ``top_ids`` (int32) and ``top_logprobs``
+    (float32), [R, k] both, receive the first k tokens of that order (k up to ``TOP_LOGPROBS_MOST``).
+
+    A token whose logit is -inf has probability zero and the log probability -inf. A logit that is not a number comes last in the
+    order. A row without a distribution (one that holds +inf or something that is no number, or nothing but -inf) gets no number for
+    all log probabilities and the entropy. A target outside the vocabulary gets no number, and the rank -1."""
+    what = "token_logprobs"
+    if not isinstance(logits, torch.Tensor) or not logits.is_cuda:
+        raise KernelError(f"{what} logits: expected a CUDA tensor")
+    if logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1) or (logits.shape[0] > 1 and logits.stride(0) < logits.shape[1]):
+        raise KernelError(f"{what} logits: expected rows of consecutive values, got shape {tuple(logits.shape)}, strides {logits.stride()}")
+    code = _code(logits, f"{what} logits")
+    R, V = logits.shape
+    _want(targets, f"{what} targets", torch.int32, 1)
+    _want(logprob, f"{what} logprob", torch.float32, 1)
+    _want(entropy, f"{what} entropy", torch.float32, 1)
+    _want(rank, f"{what} rank", torch.int32, 1)
+    top = 0
+    if (top_ids is None) != (top_logprobs is None):
+        raise KernelError(f"{what}: top_ids and top_logprobs go together")
+    if top_ids is not None:
+        _want(top_ids, f"{what} top_ids", torch.int32, 2)
+        _want(top_logprobs, f"{what} top_logprobs", torch.float32, 2)
+        top = top_ids.shape[1]
+        if top_ids.shape != (R, top) or top_logprobs.shape != (R, top):
+            raise KernelError(f"{what}: top_ids {tuple(top_ids.shape)}, top_logprobs {tuple(top_logprobs.shape)} for {R} rows")
+    if targets.numel() != R or logprob.numel() != R or entropy.numel() != R or rank.numel() != R:
+        raise KernelError(f"{what}: {R} rows, {targets.numel()} targets, outputs of {logprob.numel()}, {entropy.numel()}, {rank.numel()}")
+    if V == 0 or top > min(V, TOP_LOGPROBS_MOST):
+        raise KernelError(f"{what}: the {top} most likely of {V} tokens (at most {TOP_LOGPROBS_MOST})")
+    _on_current_device(what, logits, targets, logprob, entropy, rank, top_ids, top_logprobs)
+    if R == 0:
+        return
+    lib = library("scoring")
+    _check(lib, lib.lp_token_logprobs(logits.data_ptr(), code, logits.stride(0) if R > 1 else V, targets.data_ptr(), logprob.data_ptr(),
+                                      entropy.data_ptr(), rank.data_ptr(), _ptr(top_ids), _ptr(top_logprobs), R, V, top, _stream()))
