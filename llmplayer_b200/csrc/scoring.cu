@@ -5,102 +5,369 @@
 //   rank = how many tokens come before t in the order of falling logits (equal logits: the lower token first; a logit that
 //   is not a number comes behind all others), and the first k tokens of that order with their log probabilities.
 // Sums are taken against the row's maximum m over the others only: with c logits equal to m and r = sum of exp(x[i] - m) over
-// the rest, ln(sum) = m + ln(c + r) is formed as log1p(c - 1 + r), so that a nearly certain token's log probability keeps its digits.
+// the rest, ln(sum) = m + ln(c + r) is formed as log1p(c - 1 + r), so that a nearly certain token's log probability keeps its
+// digits; the entropy is ln(c + r) - u / (c + r) with u = sum of (x[i] - m) exp(x[i] - m).
 // A row without a distribution (it holds +inf or no number at all, or nothing but -inf) gets no number everywhere but in ranks and tokens.
+//
+// A row is read once. Every thread keeps (m, c, r, u) of what it has seen and brings the sums down when its maximum moves; a
+// warp keeps its k first tokens sorted over its lanes, and a logit is looked at again only if it is not below the best k-th
+// logit that any warp of the CTA has. A cluster of CTAs shares a long row when the rows are few; their parts meet in the first CTA's
+// registers through distributed shared memory, so there is no scratch in memory and no order of arrival: results repeat bit for bit.
 #include "common.cuh"
 
 namespace {
 
-constexpr int THREADS = 512;
+constexpr int THREADS = 256;
+constexpr int WARPS = THREADS / 32;
+constexpr int CTAS_PER_SM = 3;
 constexpr int MOST_TOP = 32;
+constexpr int MOST_CLUSTER = 8;
+constexpr int VALUES = 16;                       // logits that a thread has in hand at a time
+constexpr uint32_t ALL = 0xffffffffu;
 
-// x before y in the order of the tokens
-__device__ __forceinline__ bool before(float x, int i, float y, int j) {
-    const bool nx = x != x, ny = y != y;
-    if (nx || ny) return nx == ny ? i < j : ny;
-    return x > y || (x == y && i < j);
+// ------------------------------------------------------------------ the order of the tokens
+// A logit as an unsigned number of the same order (both zeros alike, no number below everything), and with its token: the larger
+// comes first. 0 is nobody.
+__device__ __forceinline__ uint32_t order_key(float x) {
+    const uint32_t u = __float_as_uint(x + 0.0f);
+    return x != x ? 0u : ((int)u < 0 ? ~u : u | 0x80000000u);
+}
+__device__ __forceinline__ float key_value(uint32_t k) {
+    return k == 0 ? __uint_as_float(0x7fffffffu) : __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
+}
+__device__ __forceinline__ uint64_t entry(float x, int i) { return ((uint64_t)order_key(x) << 32) | (uint32_t)~i; }
+__device__ __forceinline__ bool before(float x, int i, float y, int j) { return entry(x, i) > entry(y, j); }
+
+// 32 entries, one per lane, in falling order
+__device__ __forceinline__ uint64_t sort32(uint64_t v, int lane) {
+#pragma unroll
+    for (int size = 2; size <= 32; size <<= 1)
+#pragma unroll
+        for (int stride = size >> 1; stride > 0; stride >>= 1) {
+            const uint64_t w = __shfl_xor_sync(ALL, v, stride);
+            const bool larger = ((lane & stride) == 0) == ((lane & size) == 0);
+            v = (v > w) == larger ? v : w;
+        }
+    return v;
+}
+// the first 32 of two sorted lists
+__device__ __forceinline__ uint64_t merge32(uint64_t a, uint64_t b, int lane) {
+    const uint64_t w = __shfl_sync(ALL, b, 31 - lane);
+    a = a > w ? a : w;
+#pragma unroll
+    for (int stride = 16; stride > 0; stride >>= 1) {
+        const uint64_t p = __shfl_xor_sync(ALL, a, stride);
+        a = (a > p) == ((lane & stride) == 0) ? a : p;
+    }
+    return a;
+}
+// the k-th largest (from 0) of 32 keys
+__device__ __forceinline__ uint32_t kth_key(uint32_t v, int k, int lane) {
+#pragma unroll
+    for (int size = 2; size <= 32; size <<= 1)
+#pragma unroll
+        for (int stride = size >> 1; stride > 0; stride >>= 1) {
+            const uint32_t w = __shfl_xor_sync(ALL, v, stride);
+            const bool larger = ((lane & stride) == 0) == ((lane & size) == 0);
+            v = larger ? max(v, w) : min(v, w);
+        }
+    return __shfl_sync(ALL, v, k);
+}
+
+// ------------------------------------------------------------------ sums against a maximum
+constexpr float LOG2E = 1.4426950408889634f;
+// the hardware's exp2: within 2^-22 of the value, and each term is rounded by as much already
+__device__ __forceinline__ float fast_exp(float d) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(d * LOG2E));
+    return y;
+}
+struct Sums {
+    float m, c, r, u;           // maximum, how often it occurs, the others' sum and weighted sum against it
+    int ahead;                  // logits before the target's
+    // The same against a larger maximum. A part that has seen nothing but -inf adds nothing, one that has seen no numbers passes that on.
+    __device__ __forceinline__ void lower(float to) {
+        const float d = fmaxf(m - to, -1e30f), f = m == to ? 1.f : expf(d), w = (m == -INFINITY ? 0.f : c) + r;
+        u = f * (u + w * d);
+        r = f * w;
+        c = 0.f;
+        m = to;
+    }
+    __device__ __forceinline__ void add(Sums o) {
+        if (o.m > m) lower(o.m);
+        else if (o.m < m) o.lower(m);
+        c += o.c;
+        r += o.r;
+        u += o.u;
+        ahead += o.ahead;
+    }
+};
+__device__ __forceinline__ Sums shuffled(const Sums& s, int o) {
+    return {__shfl_xor_sync(ALL, s.m, o), __shfl_xor_sync(ALL, s.c, o), __shfl_xor_sync(ALL, s.r, o), __shfl_xor_sync(ALL, s.u, o),
+            __shfl_xor_sync(ALL, s.ahead, o)};
+}
+
+// ------------------------------------------------------------------ loads: 16 bytes at a time, the row's ends one by one
+template <typename T> struct Vec;
+template <> struct Vec<float> {
+    static constexpr int N = 4;
+    static __device__ __forceinline__ void spread(const uint4& v, float* x) {
+        x[0] = __uint_as_float(v.x); x[1] = __uint_as_float(v.y); x[2] = __uint_as_float(v.z); x[3] = __uint_as_float(v.w);
+    }
+    static __device__ __forceinline__ uint4 gather(const float* row, int i0, int V) {
+        float x[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = i0 + e >= 0 && i0 + e < V ? row[i0 + e] : -INFINITY;
+        return make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3]));
+    }
+    static __device__ __forceinline__ uint4 nothing() { return make_uint4(0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u); }
+};
+template <> struct Vec<__nv_bfloat16> {
+    static constexpr int N = 8;
+    static __device__ __forceinline__ void spread(const uint4& v, float* x) {
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) { x[2 * e] = __uint_as_float(w[e] << 16); x[2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u); }
+    }
+    static __device__ __forceinline__ uint4 gather(const __nv_bfloat16* row, int i0, int V) {
+        uint32_t w[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int a = i0 + 2 * e, b = a + 1;
+            const uint32_t lo = a >= 0 && a < V ? __bfloat16_as_ushort(row[a]) : 0xff80u;
+            const uint32_t hi = b >= 0 && b < V ? __bfloat16_as_ushort(row[b]) : 0xff80u;
+            w[e] = lo | hi << 16;
+        }
+        return make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    static __device__ __forceinline__ uint4 nothing() { return make_uint4(0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u); }
+};
+__device__ __forceinline__ uint4 load_once(const void* p) {
+    uint4 v;
+    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
+}
+
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t remote(const void* p, int cta) {
+    uint32_t a;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(cta));
+    return a;
+}
+__device__ __forceinline__ uint32_t remote_word(uint32_t a) {
+    uint32_t v;
+    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
+    return v;
+}
+
+// What a warp, and in the end a CTA, has found.
+struct Part {
+    uint64_t list[32];
+    Sums sums;
+};
+
+// grid: (rows x cluster); the CTAs of a cluster take consecutive slices of one row.
+template <typename T, bool TOP>
+__global__ void __launch_bounds__(THREADS, CTAS_PER_SM)
+token_logprobs_kernel(const T* __restrict__ logits, long long ld, const int* __restrict__ targets, float* __restrict__ logprob,
+                      float* __restrict__ entropy, int* __restrict__ rank, int* __restrict__ top_ids, float* __restrict__ top_logprobs,
+                      int V, int top, int cluster) {
+    constexpr int N = Vec<T>::N, PER = VALUES / N;             // logits per vector, vectors in hand
+    __shared__ Part parts[WARPS];
+    __shared__ uint64_t pending[TOP ? WARPS : 1][64];           // candidates of a warp, not yet in its list
+    __shared__ uint32_t bound;                                  // no logit below this key is among the first k
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int row = blockIdx.x / cluster, share = blockIdx.x - row * cluster;
+    lp_grid_wait();
+    const T* x = logits + (long long)row * ld;
+    const int lead = (int)(((uintptr_t)x & 15) / sizeof(T));     // logits of the first vector that lie before the row
+    const int vectors = (int)(((long long)V + lead + N - 1) / N);
+    const int each = (vectors + cluster - 1) / cluster;
+    const int from = share * each, to = min(vectors, from + each);
+    auto fetch = [&](int w) {
+        if (w >= to) return Vec<T>::nothing();
+        const int i0 = w * N - lead;
+        return i0 >= 0 && i0 <= V - N ? load_once(x + i0) : Vec<T>::gather(x, i0, V);
+    };
+    uint4 next[PER];
+#pragma unroll
+    for (int p = 0; p < PER; ++p) next[p] = fetch(from + p * THREADS + threadIdx.x);
+    const int target = targets[row];
+    const bool real = target >= 0 && target < V;
+    const float xt = real ? lp_to_float(x[target]) : INFINITY;
+    // A logit comes before the target's if it is larger, and if it is equal and its token lower. -inf and what is no number are
+    // compared one by one.
+    const bool odd = !(xt > -INFINITY);
+    const float below = xt == INFINITY ? 3.402823466e38f : nextafterf(xt, -INFINITY);       // y > below: y >= xt
+    if (TOP && threadIdx.x == 0) bound = 0;
+    if (TOP) __syncthreads();
+
+    Sums s = {-INFINITY, 0.f, 0.f, 0.f, 0};
+    uint64_t list = 0, kth = 0;          // the warp's first tokens over its lanes, and the last of the first k
+    int held = 0;                        // candidates in `pending`
+    auto flush = [&]() {
+        __syncwarp();
+        uint64_t v = lane < held ? pending[warp][lane] : 0;
+        const uint64_t rest = lane + 32 < held ? pending[warp][lane + 32] : 0;
+        __syncwarp();
+        pending[warp][lane] = rest;
+        __syncwarp();
+        held = max(0, held - 32);
+        list = merge32(list, sort32(v, lane), lane);
+        kth = __shfl_sync(ALL, list, top - 1);
+        if (lane == 0) atomicMax(&bound, (uint32_t)(kth >> 32));
+    };
+    bool first = TOP;
+    for (int w0 = from; w0 < to; w0 += PER * THREADS) {
+        float v[VALUES], mx[PER];
+#pragma unroll
+        for (int p = 0; p < PER; ++p) Vec<T>::spread(next[p], v + p * N);
+#pragma unroll
+        for (int p = 0; p < PER; ++p) next[p] = fetch(w0 + (PER + p) * THREADS + threadIdx.x);
+#pragma unroll
+        for (int p = 0; p < PER; ++p) {
+            mx[p] = fmaxf(v[p * N], v[p * N + 1]);
+#pragma unroll
+            for (int e = 2; e < N; e += 2) mx[p] = fmaxf(mx[p], fmaxf(v[p * N + e], v[p * N + e + 1]));
+        }
+        float most = mx[0];
+#pragma unroll
+        for (int p = 1; p < PER; ++p) most = fmaxf(most, mx[p]);
+        if (most > s.m) s.lower(most);
+        const float ref = fmaxf(s.m, -3.402823466e38f);          // so that -inf - ref is -inf
+#pragma unroll
+        for (int j = 0; j < VALUES; ++j) {
+            const float d = v[j] - ref, e = fast_exp(d);
+            if (v[j] == s.m) s.c += 1.f;
+            else s.r += e;
+            s.u = fmaf(e, fmaxf(d, -1e30f), s.u);
+        }
+#pragma unroll
+        for (int p = 0; p < PER; ++p) {
+            const int i0 = (w0 + p * THREADS + (int)threadIdx.x) * N - lead;
+            if (odd || (i0 <= target && target < i0 + N)) {
+                if (real) {
+#pragma unroll
+                    for (int e = 0; e < N; ++e)
+                        if (i0 + e >= 0 && i0 + e < V && w0 + p * THREADS + (int)threadIdx.x < to && before(v[p * N + e], i0 + e, xt, target)) ++s.ahead;
+                }
+            } else {
+                const float over = i0 < target ? below : xt;
+#pragma unroll
+                for (int e = 0; e < N; ++e)
+                    if (v[p * N + e] > over) ++s.ahead;
+            }
+        }
+        if (TOP) {
+            // Before anything is listed: of the lanes' maxima the k-th largest has k logits that are not below it.
+            if (first) {
+                const uint32_t t = kth_key(order_key(most), top - 1, lane);
+                if (lane == 0 && t > 0x007fffffu) atomicMax(&bound, t);      // -inf may stand for no logit at all
+                first = false;
+                __syncwarp();
+            }
+            const uint32_t limit = max(*(volatile uint32_t*)&bound, (uint32_t)(kth >> 32));
+            const float cut = key_value(limit);                  // no number while all are welcome
+#pragma unroll
+            for (int p = 0; p < PER; ++p) {
+                if (!__any_sync(ALL, !(mx[p] < cut))) continue;
+                const int at = w0 + p * THREADS + (int)threadIdx.x, i0 = at * N - lead;
+#pragma unroll
+                for (int e = 0; e < N; ++e) {
+                    const uint64_t mine = entry(v[p * N + e], i0 + e);
+                    const bool in = (uint32_t)(mine >> 32) >= limit && mine > kth && i0 + e >= 0 && i0 + e < V && at < to;
+                    const uint32_t who = __ballot_sync(ALL, in);
+                    if (who) {
+                        if (in) pending[warp][held + __popc(who & ((1u << lane) - 1))] = mine;
+                        held += __popc(who);
+                        if (held >= 32) flush();
+                    }
+                }
+            }
+        }
+    }
+    if (TOP && held > 0) flush();
+    lp_grid_release();
+
+    // ---------------------------------------------------------------- the warps' parts, then the CTAs'
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) s.add(shuffled(s, o));
+    if (lane == 0) parts[warp].sums = s;
+    if (TOP) parts[warp].list[lane] = list;
+    __syncthreads();
+    if (warp == 0) {
+        for (int w = 1; w < WARPS; ++w) {
+            s.add(parts[w].sums);
+            if (TOP) list = merge32(list, parts[w].list[lane], lane);
+        }
+        __syncwarp();
+        if (lane == 0) parts[0].sums = s;
+        if (TOP) parts[0].list[lane] = list;
+    }
+    if (cluster > 1) {
+        cluster_sync();
+        if (share == 0 && warp == 0) {
+            for (int cta = 1; cta < cluster; ++cta) {
+                const uint32_t a = remote(&parts[0].sums, cta);
+                s.add({__uint_as_float(remote_word(a)), __uint_as_float(remote_word(a + 4)), __uint_as_float(remote_word(a + 8)),
+                       __uint_as_float(remote_word(a + 12)), (int)remote_word(a + 16)});
+                if (TOP) {
+                    const uint32_t l = remote(&parts[0].list[lane], cta);
+                    list = merge32(list, (uint64_t)remote_word(l + 4) << 32 | remote_word(l), lane);
+                }
+            }
+        }
+        cluster_sync();                                          // the others' shared memory stays until it has been read
+    }
+    if (share == 0 && warp == 0) {
+        const bool none = !(s.m > -INFINITY && s.m < INFINITY) || s.r != s.r;
+        const float log_s = none ? NAN : log1pf((s.c - 1.f) + s.r);
+        if (lane == 0) {
+            logprob[row] = real ? (xt - s.m) - log_s : NAN;
+            entropy[row] = log_s - s.u / (s.c + s.r);
+            rank[row] = real ? s.ahead : -1;
+        }
+        if (TOP && lane < top) {
+            top_ids[(long long)row * top + lane] = (int)~(uint32_t)list;
+            top_logprobs[(long long)row * top + lane] = (key_value((uint32_t)(list >> 32)) - s.m) - log_s;
+        }
+    }
 }
 
 template <typename T>
-__global__ void __launch_bounds__(THREADS)
-token_logprobs_kernel(const T* __restrict__ logits, long long ld, const int* __restrict__ targets, float* __restrict__ logprob,
-                      float* __restrict__ entropy, int* __restrict__ rank, int* __restrict__ top_ids, float* __restrict__ top_logprobs,
-                      int V, int top) {
-    __shared__ float scratch[32];
-    __shared__ int best_at[32];
-    lp_grid_wait();
-    lp_grid_release();
-    const T* x = logits + (long long)blockIdx.x * ld;
-    const int target = targets[blockIdx.x];
-    const bool real = target >= 0 && target < V;
-    const float xt = real ? lp_to_float(x[target]) : 0.f;
-    float m = -INFINITY;
-    for (int i = threadIdx.x; i < V; i += THREADS) m = fmaxf(m, lp_to_float(x[i]));
-    m = lp_block_max(m, scratch);
-    float c = 0.f, r = 0.f, u = 0.f, ahead = 0.f;
-    for (int i = threadIdx.x; i < V; i += THREADS) {
-        const float v = lp_to_float(x[i]);
-        if (v == m) c += 1.f;
-        else {
-            const float d = v - m, e = expf(d);
-            r += e;
-            if (e != 0.f) u += e * d;
-        }
-        if (real && before(v, i, xt, target)) ahead += 1.f;
-    }
-    c = lp_block_sum(c, scratch);
-    r = lp_block_sum(r, scratch);
-    u = lp_block_sum(u, scratch);
-    ahead = lp_block_sum(ahead, scratch);
-    const bool none = !(m > -INFINITY && m < INFINITY) || r != r;
-    const float log_s = none ? NAN : log1pf((c - 1.f) + r);
-    if (threadIdx.x == 0) {
-        logprob[blockIdx.x] = real ? (xt - m) - log_s : NAN;
-        entropy[blockIdx.x] = log_s - u / (c + r);
-        rank[blockIdx.x] = real ? (int)ahead : -1;
-    }
-    float last = INFINITY;
-    int last_at = -1;
-    for (int k = 0; k < top; ++k) {                     // the first token behind the last one found
-        float v = NAN;
-        int at = V;
-        for (int i = threadIdx.x; i < V; i += THREADS) {
-            const float w = lp_to_float(x[i]);
-            if ((k == 0 || before(last, last_at, w, i)) && (at == V || before(w, i, v, at))) { v = w; at = i; }
-        }
-        for (int o = 16; o > 0; o >>= 1) {
-            const float w = __shfl_xor_sync(0xffffffffu, v, o);
-            const int j = __shfl_xor_sync(0xffffffffu, at, o);
-            if (j < V && (at == V || before(w, j, v, at))) { v = w; at = j; }
-        }
-        __syncthreads();
-        if ((threadIdx.x & 31) == 0) { scratch[threadIdx.x >> 5] = v; best_at[threadIdx.x >> 5] = at; }
-        __syncthreads();
-        for (int w = 0; w < THREADS / 32; ++w)
-            if (best_at[w] < V && (at == V || before(scratch[w], best_at[w], v, at))) { v = scratch[w]; at = best_at[w]; }
-        last = v;
-        last_at = at;
-        if (threadIdx.x == 0) {
-            top_ids[(long long)blockIdx.x * top + k] = at;
-            top_logprobs[(long long)blockIdx.x * top + k] = (v - m) - log_s;
-        }
-    }
+int launch(const void* logits, long long ld, const int* targets, float* logprob, float* entropy, int* rank, int* top_ids, float* top_logprobs,
+           int rows, int V, int top, int cluster, cudaStream_t stream) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(rows * cluster));
+    cfg.blockDim = dim3(THREADS);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = cluster;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = lp_pdl_enabled() ? 2 : 1;
+    cudaLaunchKernelEx(&cfg, top ? token_logprobs_kernel<T, true> : token_logprobs_kernel<T, false>, (const T*)logits, ld, targets, logprob, entropy,
+                       rank, top_ids, top_logprobs, V, top, cluster);
+    return lp_check_launch("token_logprobs");
 }
 
 }  // namespace
-
-extern "C" int lp_token_logprobs_most_top() { return MOST_TOP; }
 
 // logits: rows of `ld` elements (float32 or bfloat16); targets, rank int32 [rows]; logprob, entropy float32 [rows];
 // top_ids int32, top_logprobs float32 [rows, top] (null for top == 0).
 extern "C" int lp_token_logprobs(const void* logits, int dtype, long long ld, const int* targets, float* logprob, float* entropy, int* rank,
                                  int* top_ids, float* top_logprobs, int rows, int V, int top, cudaStream_t stream) {
-    if (rows <= 0 || V <= 0 || top < 0 || top > MOST_TOP || top > V || ld < V) LP_REFUSE("token_logprobs: %d rows of %d logits, the %d most likely", rows, V, top);
+    if (rows <= 0 || V <= 0 || top < 0 || top > MOST_TOP || top > V || ld < V || rows > 0x7fffffff / MOST_CLUSTER || V > 0x7fffffff - 4 * THREADS * VALUES)
+        LP_REFUSE("token_logprobs: %d rows of %d logits, the %d most likely", rows, V, top);
+    // few rows: as many CTAs per row as the GPU holds at once, each with a whole load of its threads at least
+    int cluster = 1;
+    while (cluster < MOST_CLUSTER && (long long)rows * cluster * 2 <= (long long)lp_sm_count() * CTAS_PER_SM && V / (cluster * 2) >= THREADS * VALUES / 2) cluster *= 2;
     if (dtype == LP_F32)
-        lp_launch(token_logprobs_kernel<float>, dim3(rows), dim3(THREADS), 0, stream, (const float*)logits, ld, targets, logprob, entropy, rank,
-                  top_ids, top_logprobs, V, top);
-    else
-        lp_launch(token_logprobs_kernel<__nv_bfloat16>, dim3(rows), dim3(THREADS), 0, stream, (const __nv_bfloat16*)logits, ld, targets, logprob,
-                  entropy, rank, top_ids, top_logprobs, V, top);
-    return lp_check_launch("token_logprobs");
+        return launch<float>(logits, ld, targets, logprob, entropy, rank, top_ids, top_logprobs, rows, V, top, cluster, stream);
+    return launch<__nv_bfloat16>(logits, ld, targets, logprob, entropy, rank, top_ids, top_logprobs, rows, V, top, cluster, stream);
 }

@@ -139,7 +139,6 @@ _SIGNATURES = {
         "lp_sample_fetch": [_P, _P, _I, _I, _I, _I, _P],
     },
     "scoring": {
-        "lp_token_logprobs_most_top": [],
         "lp_token_logprobs": [_P, _I, ctypes.c_longlong, _P, _P, _P, _P, _P, _P, _I, _I, _I, _P],
     },
     "shared_prefix": {
