@@ -9,7 +9,8 @@
 // digits; the entropy is ln(c + r) - u / (c + r) with u = sum of (x[i] - m) exp(x[i] - m).
 // A row without a distribution (it holds +inf or no number at all, or nothing but -inf) gets no number everywhere but in ranks and tokens.
 //
-// A row is read once. Every thread keeps (m, c, r, u) of what it has seen and brings the sums down when its maximum moves; a
+// A row is read once. Every thread keeps (c, r, u) of what it has seen against its warp's maximum m and brings them down when that
+// moves, which it does a few times per row: only then, and where a logit is -inf, are logits compared with m one by one. A
 // warp keeps its k first tokens sorted over its lanes, and a logit is looked at again only if it is not below the best k-th
 // logit that any warp of the CTA has. A cluster of CTAs shares a long row when the rows are few; their parts meet in the first CTA's
 // registers through distributed shared memory, so there is no scratch in memory and no order of arrival: results repeat bit for bit.
@@ -77,10 +78,44 @@ __device__ __forceinline__ uint32_t kth_key(uint32_t v, int k, int lane) {
 // ------------------------------------------------------------------ sums against a maximum
 constexpr float LOG2E = 1.4426950408889634f;
 // the hardware's exp2: within 2^-22 of the value, and each term is rounded by as much already
-__device__ __forceinline__ float fast_exp(float d) {
+__device__ __forceinline__ float fast_exp2(float t) {
     float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(d * LOG2E));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(t));
     return y;
+}
+__device__ __forceinline__ float fast_exp(float d) { return fast_exp2(d * LOG2E); }
+// Two float32 operations in one instruction (Blackwell's packed forms); each half is rounded as by the scalar operation.
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+    uint64_t v;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b));
+    return v;
+}
+__device__ __forceinline__ void halves(float& a, float& b, uint64_t v) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ void add2(float& x0, float& x1, float y0, float y1) {
+    uint64_t v;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(pair(x0, x1)), "l"(pair(y0, y1)));
+    halves(x0, x1, v);
+}
+__device__ __forceinline__ void add2(float& x0, float& x1, float y) { add2(x0, x1, y, y); }
+__device__ __forceinline__ void mul2(float& z0, float& z1, float x0, float x1, float y) {
+    uint64_t v;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(pair(x0, x1)), "l"(pair(y, y)));
+    halves(z0, z1, v);
+}
+__device__ __forceinline__ void fma2(float& z0, float& z1, float x0, float x1, float y0, float y1) {      // z += x * y
+    uint64_t v;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(v) : "l"(pair(x0, x1)), "l"(pair(y0, y1)), "l"(pair(z0, z1)));
+    halves(z0, z1, v);
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+__device__ __forceinline__ float min3(float a, float b, float c) {
+    float d;
+    asm("min.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
 }
 struct Sums {
     float m, c, r, u;           // maximum, how often it occurs, the others' sum and weighted sum against it
@@ -186,14 +221,25 @@ token_logprobs_kernel(const T* __restrict__ logits, long long ld, const int* __r
     const int vectors = (int)(((long long)V + lead + N - 1) / N);
     const int each = (vectors + cluster - 1) / cluster;
     const int from = share * each, to = min(vectors, from + each);
-    auto fetch = [&](int w) {
-        if (w >= to) return Vec<T>::nothing();
-        const int i0 = w * N - lead;
-        return i0 >= 0 && i0 <= V - N ? load_once(x + i0) : Vec<T>::gather(x, i0, V);
-    };
+    // Vectors that lie wholly in the row and the share need no look at their ends.
+    const int whole_from = max(from, lead > 0 ? 1 : 0), whole_to = min(to, (int)(((long long)V + lead) / N));
+    const T* mine = x - lead + (long long)threadIdx.x * N;
     uint4 next[PER];
+    auto fetch = [&](int w0) {
+        if (w0 >= whole_from && w0 + PER * THREADS <= whole_to) {
+            const T* p0 = mine + (long long)w0 * N;
 #pragma unroll
-    for (int p = 0; p < PER; ++p) next[p] = fetch(from + p * THREADS + threadIdx.x);
+            for (int p = 0; p < PER; ++p) next[p] = load_once(p0 + p * THREADS * N);
+        } else {
+#pragma unroll
+            for (int p = 0; p < PER; ++p) {
+                const int w = w0 + p * THREADS + (int)threadIdx.x;
+                next[p] = w >= to ? Vec<T>::nothing() : (w >= whole_from && w < whole_to) ? load_once(mine + (long long)(w0 + p * THREADS) * N)
+                                                                                           : Vec<T>::gather(x, w * N - lead, V);
+            }
+        }
+    };
+    fetch(from);
     const int target = targets[row];
     const bool real = target >= 0 && target < V;
     const float xt = real ? lp_to_float(x[target]) : INFINITY;
@@ -221,43 +267,63 @@ token_logprobs_kernel(const T* __restrict__ logits, long long ld, const int* __r
     };
     bool first = TOP;
     for (int w0 = from; w0 < to; w0 += PER * THREADS) {
-        float v[VALUES], mx[PER];
+        float v[VALUES];
 #pragma unroll
         for (int p = 0; p < PER; ++p) Vec<T>::spread(next[p], v + p * N);
+        if (w0 + PER * THREADS < to) fetch(w0 + PER * THREADS);
+        float most = max3(v[0], v[1], v[2]), least = min3(v[0], v[1], v[2]);
 #pragma unroll
-        for (int p = 0; p < PER; ++p) next[p] = fetch(w0 + (PER + p) * THREADS + threadIdx.x);
-#pragma unroll
-        for (int p = 0; p < PER; ++p) {
-            mx[p] = fmaxf(v[p * N], v[p * N + 1]);
-#pragma unroll
-            for (int e = 2; e < N; e += 2) mx[p] = fmaxf(mx[p], fmaxf(v[p * N + e], v[p * N + e + 1]));
+        for (int j = 3; j + 1 < VALUES; j += 2) {
+            most = max3(most, v[j], v[j + 1]);
+            least = min3(least, v[j], v[j + 1]);
         }
-        float most = mx[0];
+        most = fmaxf(most, v[VALUES - 1]);
+        least = fminf(least, v[VALUES - 1]);
+        if (__any_sync(ALL, most >= s.m || least - s.m < -3e38f)) {
+            // a logit that reaches the warp's maximum, or one without a probability (or so low that the difference may overflow)
+            const float peak = key_value(max(__reduce_max_sync(ALL, order_key(most)), 0x007fffffu));
+            if (peak > s.m) s.lower(peak);
+            const float ref = fmaxf(s.m, -3.402823466e38f);          // so that -inf - ref is -inf
 #pragma unroll
-        for (int p = 1; p < PER; ++p) most = fmaxf(most, mx[p]);
-        if (most > s.m) s.lower(most);
-        const float ref = fmaxf(s.m, -3.402823466e38f);          // so that -inf - ref is -inf
+            for (int j = 0; j < VALUES; ++j) {
+                const float d = v[j] - ref, e = fast_exp(d);
+                if (v[j] == s.m) s.c += 1.f;
+                else s.r += e;
+                s.u = fmaf(e, fmaxf(d, -1e30f), s.u);
+            }
+        } else {
+            float r0 = 0.f, r1 = 0.f, u0 = 0.f, u1 = 0.f;
 #pragma unroll
-        for (int j = 0; j < VALUES; ++j) {
-            const float d = v[j] - ref, e = fast_exp(d);
-            if (v[j] == s.m) s.c += 1.f;
-            else s.r += e;
-            s.u = fmaf(e, fmaxf(d, -1e30f), s.u);
+            for (int j = 0; j < VALUES; j += 2) {
+                float d0 = v[j], d1 = v[j + 1], t0, t1;
+                add2(d0, d1, -s.m);
+                mul2(t0, t1, d0, d1, LOG2E);
+                t0 = fast_exp2(t0);
+                t1 = fast_exp2(t1);
+                add2(r0, r1, t0, t1);
+                fma2(u0, u1, t0, t1, d0, d1);
+            }
+            s.r += r0 + r1;
+            s.u += u0 + u1;
         }
+        // the target's rank
+        const int at0 = w0 * N - lead;                                // the first logit in the CTA's hands
+        if (odd || __any_sync(ALL, most > below) || (target >= at0 && target < at0 + PER * THREADS * N)) {
 #pragma unroll
-        for (int p = 0; p < PER; ++p) {
-            const int i0 = (w0 + p * THREADS + (int)threadIdx.x) * N - lead;
-            if (odd || (i0 <= target && target < i0 + N)) {
-                if (real) {
+            for (int p = 0; p < PER; ++p) {
+                const int w = w0 + p * THREADS + (int)threadIdx.x, i0 = w * N - lead;
+                if (odd || (i0 <= target && target < i0 + N)) {
+                    if (real) {
+#pragma unroll
+                        for (int e = 0; e < N; ++e)
+                            if (i0 + e >= 0 && i0 + e < V && w < to && before(v[p * N + e], i0 + e, xt, target)) ++s.ahead;
+                    }
+                } else {
+                    const float over = i0 < target ? below : xt;
 #pragma unroll
                     for (int e = 0; e < N; ++e)
-                        if (i0 + e >= 0 && i0 + e < V && w0 + p * THREADS + (int)threadIdx.x < to && before(v[p * N + e], i0 + e, xt, target)) ++s.ahead;
+                        if (v[p * N + e] > over) ++s.ahead;
                 }
-            } else {
-                const float over = i0 < target ? below : xt;
-#pragma unroll
-                for (int e = 0; e < N; ++e)
-                    if (v[p * N + e] > over) ++s.ahead;
             }
         }
         if (TOP) {
@@ -270,9 +336,13 @@ token_logprobs_kernel(const T* __restrict__ logits, long long ld, const int* __r
             }
             const uint32_t limit = max(*(volatile uint32_t*)&bound, (uint32_t)(kth >> 32));
             const float cut = key_value(limit);                  // no number while all are welcome
+            if (__any_sync(ALL, !(most < cut)))
 #pragma unroll
             for (int p = 0; p < PER; ++p) {
-                if (!__any_sync(ALL, !(mx[p] < cut))) continue;
+                float high = fmaxf(v[p * N], v[p * N + 1]);
+#pragma unroll
+                for (int e = 2; e < N; ++e) high = fmaxf(high, v[p * N + e]);
+                if (!__any_sync(ALL, !(high < cut))) continue;
                 const int at = w0 + p * THREADS + (int)threadIdx.x, i0 = at * N - lead;
 #pragma unroll
                 for (int e = 0; e < N; ++e) {
