@@ -11,8 +11,8 @@
 //
 // A row is read once. Every thread keeps (c, r, u) of what it has seen against its warp's maximum m and brings them down when that
 // moves, which it does a few times per row: only then, and where a logit is -inf, are logits compared with m one by one. A
-// warp keeps its k first tokens sorted over its lanes, and a logit is looked at again only if it is not below the best k-th
-// logit that any warp of the CTA has. A cluster of CTAs shares a long row when the rows are few; their parts meet in the first CTA's
+// warp keeps its k first tokens sorted over its lanes, and a logit is looked at again only if it is not below a bound that the
+// warps' largest logits so far give. A cluster of CTAs shares a long row when the rows are few; their parts meet in the first CTA's
 // registers through distributed shared memory, so there is no scratch in memory and no order of arrival: results repeat bit for bit.
 #include "common.cuh"
 
@@ -23,6 +23,7 @@ constexpr int WARPS = THREADS / 32;
 constexpr int CTAS_PER_SM = 3;
 constexpr int MOST_TOP = 32;
 constexpr int MOST_CLUSTER = 8;
+constexpr int PENDING = 64;
 constexpr int VALUES = 16;                       // logits that a thread has in hand at a time
 constexpr uint32_t ALL = 0xffffffffu;
 
@@ -39,13 +40,13 @@ __device__ __forceinline__ float key_value(uint32_t k) {
 __device__ __forceinline__ uint64_t entry(float x, int i) { return ((uint64_t)order_key(x) << 32) | (uint32_t)~i; }
 __device__ __forceinline__ bool before(float x, int i, float y, int j) { return entry(x, i) > entry(y, j); }
 
-// 32 entries, one per lane, in falling order
-__device__ __forceinline__ uint64_t sort32(uint64_t v, int lane) {
+// 32 keys or entries, one per lane, in falling order
+template <typename K> __device__ __forceinline__ K sort32(K v, int lane) {
 #pragma unroll
     for (int size = 2; size <= 32; size <<= 1)
 #pragma unroll
         for (int stride = size >> 1; stride > 0; stride >>= 1) {
-            const uint64_t w = __shfl_xor_sync(ALL, v, stride);
+            const K w = __shfl_xor_sync(ALL, v, stride);
             const bool larger = ((lane & stride) == 0) == ((lane & size) == 0);
             v = (v > w) == larger ? v : w;
         }
@@ -62,19 +63,6 @@ __device__ __forceinline__ uint64_t merge32(uint64_t a, uint64_t b, int lane) {
     }
     return a;
 }
-// the k-th largest (from 0) of 32 keys
-__device__ __forceinline__ uint32_t kth_key(uint32_t v, int k, int lane) {
-#pragma unroll
-    for (int size = 2; size <= 32; size <<= 1)
-#pragma unroll
-        for (int stride = size >> 1; stride > 0; stride >>= 1) {
-            const uint32_t w = __shfl_xor_sync(ALL, v, stride);
-            const bool larger = ((lane & stride) == 0) == ((lane & size) == 0);
-            v = larger ? max(v, w) : min(v, w);
-        }
-    return __shfl_sync(ALL, v, k);
-}
-
 // ------------------------------------------------------------------ sums against a maximum
 constexpr float LOG2E = 1.4426950408889634f;
 // the hardware's exp2: within 2^-22 of the value, and each term is rounded by as much already
@@ -210,9 +198,10 @@ token_logprobs_kernel(const T* __restrict__ logits, long long ld, const int* __r
                       float* __restrict__ entropy, int* __restrict__ rank, int* __restrict__ top_ids, float* __restrict__ top_logprobs,
                       int V, int top, int cluster) {
     constexpr int N = Vec<T>::N, PER = VALUES / N;             // logits per vector, vectors in hand
-    __shared__ Part parts[WARPS];
-    __shared__ uint64_t pending[TOP ? WARPS : 1][64];           // candidates of a warp, not yet in its list
-    __shared__ uint32_t bound;                                  // no logit below this key is among the first k
+    __shared__ Part parts[MOST_CLUSTER > WARPS ? MOST_CLUSTER : WARPS];
+    __shared__ uint64_t pending[TOP ? WARPS : 1][PENDING];       // candidates of a warp, not yet in its list
+    __shared__ float offers[TOP ? WARPS : 1][32][VALUES];
+    __shared__ uint32_t posts[WARPS];                            // each warp has `per_warp` logits that are not below this key
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int row = blockIdx.x / cluster, share = blockIdx.x - row * cluster;
     lp_grid_wait();
@@ -247,25 +236,23 @@ token_logprobs_kernel(const T* __restrict__ logits, long long ld, const int* __r
     // compared one by one.
     const bool odd = !(xt > -INFINITY);
     const float below = xt == INFINITY ? 3.402823466e38f : nextafterf(xt, -INFINITY);       // y > below: y >= xt
-    if (TOP && threadIdx.x == 0) bound = 0;
-    if (TOP) __syncthreads();
 
     Sums s = {-INFINITY, 0.f, 0.f, 0.f, 0};
     uint64_t list = 0, kth = 0;          // the warp's first tokens over its lanes, and the last of the first k
     int held = 0;                        // candidates in `pending`
-    auto flush = [&]() {
+    auto flush = [&]() {                 // up to 32 of them into the list
         __syncwarp();
-        uint64_t v = lane < held ? pending[warp][lane] : 0;
-        const uint64_t rest = lane + 32 < held ? pending[warp][lane + 32] : 0;
-        __syncwarp();
-        pending[warp][lane] = rest;
-        __syncwarp();
-        held = max(0, held - 32);
+        const int n = min(held, 32);
+        const uint64_t v = lane < n ? pending[warp][held - n + lane] : 0;
+        held -= n;
         list = merge32(list, sort32(v, lane), lane);
         kth = __shfl_sync(ALL, list, top - 1);
-        if (lane == 0) atomicMax(&bound, (uint32_t)(kth >> 32));
+        __syncwarp();
     };
-    bool first = TOP;
+    const int per_warp = (top + WARPS - 1) / WARPS, warps_needed = per_warp ? (top + per_warp - 1) / per_warp : 0;
+    uint32_t bound = 0;                  // no logit below this key is among the first k
+    float cut = key_value(0), lane_most = -INFINITY;
+    int turn = 0;
     for (int w0 = from; w0 < to; w0 += PER * THREADS) {
         float v[VALUES];
 #pragma unroll
@@ -327,34 +314,57 @@ token_logprobs_kernel(const T* __restrict__ logits, long long ld, const int* __r
             }
         }
         if (TOP) {
-            // Before anything is listed: of the lanes' maxima the k-th largest has k logits that are not below it.
-            if (first) {
-                const uint32_t t = kth_key(order_key(most), top - 1, lane);
-                if (lane == 0 && t > 0x007fffffu) atomicMax(&bound, t);      // -inf may stand for no logit at all
-                first = false;
-                __syncwarp();
-            }
-            const uint32_t limit = max(*(volatile uint32_t*)&bound, (uint32_t)(kth >> 32));
-            const float cut = key_value(limit);                  // no number while all are welcome
-            if (__any_sync(ALL, !(most < cut)))
+            lane_most = fmaxf(lane_most, most);
+            if ((turn & (turn + 1)) == 0) {
+                // Of the lanes' largest logits so far the k-th largest has k logits that are not below it. And each warp posts a key that
+                // per_warp of its lanes are not below: what is not above enough warps' keys is not above k logits. Posts only rise, so an
+                // old one holds as well. (-inf may stand for no logit at all.)
+                const uint32_t key = order_key(lane_most);
+                const uint32_t sorted = sort32(key > 0x007fffffu ? key : 0u, lane), mine = __shfl_sync(ALL, sorted, per_warp - 1);
+                bound = max(bound, __shfl_sync(ALL, sorted, top - 1));
+                volatile uint32_t* const posted = posts;
+                if (lane == 0) posted[warp] = mine;
+                if (turn == 0) __syncthreads();
+                const uint32_t post = lane < WARPS ? posted[lane] : 0u;
+                int place = 0;
 #pragma unroll
-            for (int p = 0; p < PER; ++p) {
-                float high = fmaxf(v[p * N], v[p * N + 1]);
-#pragma unroll
-                for (int e = 2; e < N; ++e) high = fmaxf(high, v[p * N + e]);
-                if (!__any_sync(ALL, !(high < cut))) continue;
-                const int at = w0 + p * THREADS + (int)threadIdx.x, i0 = at * N - lead;
-#pragma unroll
-                for (int e = 0; e < N; ++e) {
-                    const uint64_t mine = entry(v[p * N + e], i0 + e);
-                    const bool in = (uint32_t)(mine >> 32) >= limit && mine > kth && i0 + e >= 0 && i0 + e < V && at < to;
-                    const uint32_t who = __ballot_sync(ALL, in);
-                    if (who) {
-                        if (in) pending[warp][held + __popc(who & ((1u << lane) - 1))] = mine;
-                        held += __popc(who);
-                        if (held >= 32) flush();
-                    }
+                for (int w = 0; w < WARPS; ++w) {
+                    const uint32_t other = __shfl_sync(ALL, post, w);
+                    if (other > post || (other == post && w < lane)) ++place;
                 }
+                const uint32_t who = __ballot_sync(ALL, lane < WARPS && place == warps_needed - 1);
+                bound = max(bound, __shfl_sync(ALL, post, __ffs(who) - 1));
+                cut = key_value(max(bound, (uint32_t)(kth >> 32)));
+            }
+            ++turn;
+            uint32_t who = __ballot_sync(ALL, !(most < cut));
+            if (who) {
+                // The lanes with something to offer lay out what they hold, and the warp goes through two lanes' logits at a time.
+                if (!(most < cut)) {
+#pragma unroll
+                    for (int j = 0; j < VALUES; j += 4)
+                        *reinterpret_cast<float4*>(&offers[warp][lane][j]) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+                }
+                __syncwarp();
+                while (who) {
+                    const int a = __ffs(who) - 1;
+                    who &= who - 1;
+                    const int b = who ? __ffs(who) - 1 : -1;
+                    who &= who - 1;
+                    const int from_lane = lane < 16 ? a : b, j = lane & 15;
+                    uint64_t mine = 0;
+                    if (from_lane >= 0) {
+                        const int w = w0 + j / N * THREADS + warp * 32 + from_lane, i = w * N - lead + j % N;
+                        if (i >= 0 && i < V && w < to) mine = entry(offers[warp][from_lane][j], i);
+                    }
+                    const bool in = mine > kth && (uint32_t)(mine >> 32) >= bound;
+                    const uint32_t all = __ballot_sync(ALL, in);
+                    if (in) pending[warp][held + __popc(all & ((1u << lane) - 1))] = mine;
+                    held += __popc(all);
+                    if (held >= 32) flush();
+                }
+                __syncwarp();
+                cut = key_value(max(bound, (uint32_t)(kth >> 32)));
             }
         }
     }
@@ -365,28 +375,48 @@ token_logprobs_kernel(const T* __restrict__ logits, long long ld, const int* __r
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) s.add(shuffled(s, o));
     if (lane == 0) parts[warp].sums = s;
-    if (TOP) parts[warp].list[lane] = list;
-    __syncthreads();
-    if (warp == 0) {
-        for (int w = 1; w < WARPS; ++w) {
-            s.add(parts[w].sums);
-            if (TOP) list = merge32(list, parts[w].list[lane], lane);
+    const Sums nothing = {-INFINITY, 0.f, 0.f, 0.f, 0};
+    auto lists_meet = [&](int count) {                           // the first `count` warps' lists, in warp 0's registers
+        for (int o = count / 2; o > 0; o >>= 1) {
+            if (warp >= o && warp < 2 * o) parts[warp].list[lane] = list;
+            __syncthreads();
+            if (warp < o) list = merge32(list, parts[warp + o].list[lane], lane);
         }
-        __syncwarp();
-        if (lane == 0) parts[0].sums = s;
-        if (TOP) parts[0].list[lane] = list;
+    };
+    auto sums_meet = [&]() {                                     // those of the first lanes, in all lanes
+#pragma unroll
+        for (int o = WARPS / 2; o > 0; o >>= 1) s.add(shuffled(s, o));
+        s = {__shfl_sync(ALL, s.m, 0), __shfl_sync(ALL, s.c, 0), __shfl_sync(ALL, s.r, 0), __shfl_sync(ALL, s.u, 0), __shfl_sync(ALL, s.ahead, 0)};
+    };
+    if (TOP) lists_meet(WARPS);
+    else __syncthreads();
+    if (warp == 0) {
+        s = lane < WARPS ? parts[lane].sums : nothing;
+        sums_meet();
     }
     if (cluster > 1) {
+        __syncthreads();
+        if (warp == 0) {
+            if (lane == 0) parts[0].sums = s;
+            if (TOP) parts[0].list[lane] = list;
+        }
         cluster_sync();
-        if (share == 0 && warp == 0) {
-            for (int cta = 1; cta < cluster; ++cta) {
-                const uint32_t a = remote(&parts[0].sums, cta);
-                s.add({__uint_as_float(remote_word(a)), __uint_as_float(remote_word(a + 4)), __uint_as_float(remote_word(a + 8)),
-                       __uint_as_float(remote_word(a + 12)), (int)remote_word(a + 16)});
-                if (TOP) {
-                    const uint32_t l = remote(&parts[0].list[lane], cta);
-                    list = merge32(list, (uint64_t)remote_word(l + 4) << 32 | remote_word(l), lane);
+        if (share == 0) {
+            if (warp == 0) {
+                s = nothing;
+                if (lane < cluster) {
+                    const uint32_t a = remote(&parts[0].sums, lane);
+                    s = {__uint_as_float(remote_word(a)), __uint_as_float(remote_word(a + 4)), __uint_as_float(remote_word(a + 8)),
+                         __uint_as_float(remote_word(a + 12)), (int)remote_word(a + 16)};
                 }
+                sums_meet();
+            }
+            if (TOP) {
+                if (warp < cluster) {
+                    const uint32_t a = remote(&parts[0].list[lane], warp);
+                    list = (uint64_t)remote_word(a + 4) << 32 | remote_word(a);
+                }
+                lists_meet(cluster);
             }
         }
         cluster_sync();                                          // the others' shared memory stays until it has been read
