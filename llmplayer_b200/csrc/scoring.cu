@@ -16,6 +16,8 @@
 // registers through distributed shared memory, so there is no scratch in memory and no order of arrival: results repeat bit for bit.
 #include "common.cuh"
 
+#include <type_traits>
+
 namespace {
 
 constexpr int THREADS = 256;
@@ -185,11 +187,13 @@ __device__ __forceinline__ uint32_t remote_word(uint32_t a) {
     return v;
 }
 
-// What a warp, and in the end a CTA, has found.
-struct Part {
-    uint64_t list[32];
-    Sums sums;
+// The candidates of a CTA (in the first CTA of a cluster: of all) and the first k of them; its sums.
+struct Found {
+    __align__(16) uint64_t pool[WARPS * (MOST_TOP + PENDING)];
+    uint64_t best[MOST_TOP];
+    int count;
 };
+static_assert(WARPS * (MOST_TOP + PENDING) >= MOST_CLUSTER * MOST_TOP && MOST_CLUSTER <= 32 && WARPS <= 32, "one lane per part, room for all lists");
 
 // grid: (rows x cluster); the CTAs of a cluster take consecutive slices of one row.
 template <typename T, bool TOP>
@@ -198,9 +202,11 @@ token_logprobs_kernel(const T* __restrict__ logits, long long ld, const int* __r
                       float* __restrict__ entropy, int* __restrict__ rank, int* __restrict__ top_ids, float* __restrict__ top_logprobs,
                       int V, int top, int cluster) {
     constexpr int N = Vec<T>::N, PER = VALUES / N;             // logits per vector, vectors in hand
-    __shared__ Part parts[MOST_CLUSTER > WARPS ? MOST_CLUSTER : WARPS];
+    __shared__ Sums parts[WARPS];
+    __shared__ Sums whole;
+    __shared__ Found found;
     __shared__ uint64_t pending[TOP ? WARPS : 1][PENDING];       // candidates of a warp, not yet in its list
-    __shared__ float offers[TOP ? WARPS : 1][32][VALUES];
+    __shared__ __align__(16) float offers[TOP ? WARPS : 1][32][VALUES];
     __shared__ uint32_t posts[WARPS];                            // each warp has `per_warp` logits that are not below this key
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int row = blockIdx.x / cluster, share = blockIdx.x - row * cluster;
@@ -232,10 +238,7 @@ token_logprobs_kernel(const T* __restrict__ logits, long long ld, const int* __r
     const int target = targets[row];
     const bool real = target >= 0 && target < V;
     const float xt = real ? lp_to_float(x[target]) : INFINITY;
-    // A logit comes before the target's if it is larger, and if it is equal and its token lower. -inf and what is no number are
-    // compared one by one.
-    const bool odd = !(xt > -INFINITY);
-    const float below = xt == INFINITY ? 3.402823466e38f : nextafterf(xt, -INFINITY);       // y > below: y >= xt
+    // A logit comes before the target's if it is larger, and if it is equal and its token lower.
 
     Sums s = {-INFINITY, 0.f, 0.f, 0.f, 0};
     uint64_t list = 0, kth = 0;          // the warp's first tokens over its lanes, and the last of the first k
@@ -266,8 +269,26 @@ token_logprobs_kernel(const T* __restrict__ logits, long long ld, const int* __r
         }
         most = fmaxf(most, v[VALUES - 1]);
         least = fminf(least, v[VALUES - 1]);
-        if (__any_sync(ALL, most >= s.m || least - s.m < -3e38f)) {
-            // a logit that reaches the warp's maximum, or one without a probability (or so low that the difference may overflow)
+        // Against the warp's maximum, two logits at a time. Where a logit is -inf (or so low that the difference overflows) the
+        // weighted sum takes its term, zero times that, against a finite difference.
+        auto add_up = [&](auto masked) {
+            float r0 = 0.f, r1 = 0.f, u0 = 0.f, u1 = 0.f;
+#pragma unroll
+            for (int j = 0; j < VALUES; j += 2) {
+                float d0 = v[j], d1 = v[j + 1], t0, t1;
+                add2(d0, d1, -s.m);
+                mul2(t0, t1, d0, d1, LOG2E);
+                t0 = fast_exp2(t0);
+                t1 = fast_exp2(t1);
+                add2(r0, r1, t0, t1);
+                if (masked.value) { d0 = fmaxf(d0, -1e30f); d1 = fmaxf(d1, -1e30f); }
+                fma2(u0, u1, t0, t1, d0, d1);
+            }
+            s.r += r0 + r1;
+            s.u += u0 + u1;
+        };
+        if (__any_sync(ALL, most >= s.m)) {
+            // a logit that reaches the warp's maximum: one by one
             const float peak = key_value(max(__reduce_max_sync(ALL, order_key(most)), 0x007fffffu));
             if (peak > s.m) s.lower(peak);
             const float ref = fmaxf(s.m, -3.402823466e38f);          // so that -inf - ref is -inf
@@ -278,45 +299,36 @@ token_logprobs_kernel(const T* __restrict__ logits, long long ld, const int* __r
                 else s.r += e;
                 s.u = fmaf(e, fmaxf(d, -1e30f), s.u);
             }
-        } else {
-            float r0 = 0.f, r1 = 0.f, u0 = 0.f, u1 = 0.f;
-#pragma unroll
-            for (int j = 0; j < VALUES; j += 2) {
-                float d0 = v[j], d1 = v[j + 1], t0, t1;
-                add2(d0, d1, -s.m);
-                mul2(t0, t1, d0, d1, LOG2E);
-                t0 = fast_exp2(t0);
-                t1 = fast_exp2(t1);
-                add2(r0, r1, t0, t1);
-                fma2(u0, u1, t0, t1, d0, d1);
-            }
-            s.r += r0 + r1;
-            s.u += u0 + u1;
-        }
+        } else if (__any_sync(ALL, least - s.m < -3e38f)) add_up(std::true_type());
+        else add_up(std::false_type());
         // the target's rank
         const int at0 = w0 * N - lead;                                // the first logit in the CTA's hands
-        if (odd || __any_sync(ALL, most > below) || (target >= at0 && target < at0 + PER * THREADS * N)) {
+        if (__any_sync(ALL, !(most < xt)) || (target >= at0 && target < at0 + PER * THREADS * N)) {
 #pragma unroll
             for (int p = 0; p < PER; ++p) {
                 const int w = w0 + p * THREADS + (int)threadIdx.x, i0 = w * N - lead;
-                if (odd || (i0 <= target && target < i0 + N)) {
+                // one by one: around the target, against no number, and against -inf where not all are logits of the row
+                if (xt != xt || (i0 <= target && target < i0 + N) || (xt == -INFINITY && !(w >= whole_from && w < whole_to))) {
                     if (real) {
 #pragma unroll
                         for (int e = 0; e < N; ++e)
                             if (i0 + e >= 0 && i0 + e < V && w < to && before(v[p * N + e], i0 + e, xt, target)) ++s.ahead;
                     }
-                } else {
-                    const float over = i0 < target ? below : xt;
+                } else if (i0 < target) {
 #pragma unroll
                     for (int e = 0; e < N; ++e)
-                        if (v[p * N + e] > over) ++s.ahead;
+                        if (v[p * N + e] >= xt) ++s.ahead;
+                } else {
+#pragma unroll
+                    for (int e = 0; e < N; ++e)
+                        if (v[p * N + e] > xt) ++s.ahead;
                 }
             }
         }
         if (TOP) {
             lane_most = fmaxf(lane_most, most);
-            if ((turn & (turn + 1)) == 0) {
-                // Of the lanes' largest logits so far the k-th largest has k logits that are not below it. And each warp posts a key that
+            if ((turn & (turn + 1)) == 0 && (turn == 0 || to - w0 > turn * PER * THREADS)) {
+                // At first, and whenever as much has been seen again as before and most is still to come: of the lanes' largest logits so far the k-th largest has k logits that are not below it. And each warp posts a key that
                 // per_warp of its lanes are not below: what is not above enough warps' keys is not above k logits. Posts only rise, so an
                 // old one holds as well. (-inf may stand for no logit at all.)
                 const uint32_t key = order_key(lane_most);
@@ -368,71 +380,96 @@ token_logprobs_kernel(const T* __restrict__ logits, long long ld, const int* __r
             }
         }
     }
-    if (TOP && held > 0) flush();
     lp_grid_release();
 
     // ---------------------------------------------------------------- the warps' parts, then the CTAs'
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) s.add(shuffled(s, o));
-    if (lane == 0) parts[warp].sums = s;
+    if (lane == 0) parts[warp] = s;
+    if (TOP && threadIdx.x == 0) found.count = 0;
+    __syncthreads();
     const Sums nothing = {-INFINITY, 0.f, 0.f, 0.f, 0};
-    auto lists_meet = [&](int count) {                           // the first `count` warps' lists, in warp 0's registers
-        for (int o = count / 2; o > 0; o >>= 1) {
-            if (warp >= o && warp < 2 * o) parts[warp].list[lane] = list;
-            __syncthreads();
-            if (warp < o) list = merge32(list, parts[warp + o].list[lane], lane);
-        }
-    };
-    auto sums_meet = [&]() {                                     // those of the first lanes, in all lanes
+    auto sums_meet = [&]() {                                     // those of a warp's lanes, in all of them
 #pragma unroll
-        for (int o = WARPS / 2; o > 0; o >>= 1) s.add(shuffled(s, o));
-        s = {__shfl_sync(ALL, s.m, 0), __shfl_sync(ALL, s.c, 0), __shfl_sync(ALL, s.r, 0), __shfl_sync(ALL, s.u, 0), __shfl_sync(ALL, s.ahead, 0)};
+        for (int o = 16; o > 0; o >>= 1) s.add(shuffled(s, o));
     };
-    if (TOP) lists_meet(WARPS);
-    else __syncthreads();
     if (warp == 0) {
-        s = lane < WARPS ? parts[lane].sums : nothing;
+        s = lane < WARPS ? parts[lane] : nothing;
         sums_meet();
+        if (lane == 0) whole = s;
+    }
+    // A candidate's place is the number of candidates before it: no sorting, and the order in which they lie does not matter.
+    auto place_of = [&](uint64_t mine, int n) {
+        int place = 0;
+#pragma unroll 4
+        for (int i = 0; i < n; i += 2) {
+            const ulonglong2 two = *reinterpret_cast<const ulonglong2*>(&found.pool[i]);
+            place += (two.x > mine ? 1 : 0) + (two.y > mine && i + 1 < n ? 1 : 0);
+        }
+        return place;
+    };
+    int candidates = 0;
+    if (TOP) {
+        const uint32_t listed = __ballot_sync(ALL, list != 0 && lane < top);
+        int at = 0;
+        if (lane == 0) at = atomicAdd(&found.count, __popc(listed) + held);
+        at = __shfl_sync(ALL, at, 0);
+        if (list != 0 && lane < top) found.pool[at + lane] = list;
+        at += __popc(listed);
+        __syncwarp();
+        for (int i = lane; i < held; i += 32) found.pool[at + i] = pending[warp][i];
+        if (warp == 0) found.best[lane] = 0;
+        __syncthreads();
+        candidates = found.count;
     }
     if (cluster > 1) {
-        __syncthreads();
-        if (warp == 0) {
-            if (lane == 0) parts[0].sums = s;
-            if (TOP) parts[0].list[lane] = list;
-        }
+        if (TOP)
+            for (int i = threadIdx.x; i < candidates; i += THREADS) {
+                const uint64_t mine = found.pool[i];
+                const int place = place_of(mine, candidates);
+                if (place < top) found.best[place] = mine;
+            }
         cluster_sync();
         if (share == 0) {
             if (warp == 0) {
                 s = nothing;
                 if (lane < cluster) {
-                    const uint32_t a = remote(&parts[0].sums, lane);
+                    const uint32_t a = remote(&whole, lane);
                     s = {__uint_as_float(remote_word(a)), __uint_as_float(remote_word(a + 4)), __uint_as_float(remote_word(a + 8)),
                          __uint_as_float(remote_word(a + 12)), (int)remote_word(a + 16)};
                 }
                 sums_meet();
+                __syncwarp();
+                if (lane == 0) whole = s;                        // nobody else reads this CTA's
             }
             if (TOP) {
-                if (warp < cluster) {
-                    const uint32_t a = remote(&parts[0].list[lane], warp);
-                    list = (uint64_t)remote_word(a + 4) << 32 | remote_word(a);
+                candidates = cluster * top;
+                for (int i = threadIdx.x; i < candidates; i += THREADS) {
+                    const uint32_t a = remote(&found.best[i % top], i / top);
+                    found.pool[i] = (uint64_t)remote_word(a + 4) << 32 | remote_word(a);
                 }
-                lists_meet(cluster);
             }
         }
         cluster_sync();                                          // the others' shared memory stays until it has been read
-    }
-    if (share == 0 && warp == 0) {
+    } else __syncthreads();
+    if (share == 0) {
+        s = whole;
         const bool none = !(s.m > -INFINITY && s.m < INFINITY) || s.r != s.r;
         const float log_s = none ? NAN : log1pf((s.c - 1.f) + s.r);
-        if (lane == 0) {
+        if (threadIdx.x == 0) {
             logprob[row] = real ? (xt - s.m) - log_s : NAN;
             entropy[row] = log_s - s.u / (s.c + s.r);
             rank[row] = real ? s.ahead : -1;
         }
-        if (TOP && lane < top) {
-            top_ids[(long long)row * top + lane] = (int)~(uint32_t)list;
-            top_logprobs[(long long)row * top + lane] = (key_value((uint32_t)(list >> 32)) - s.m) - log_s;
-        }
+        if (TOP)
+            for (int i = threadIdx.x; i < candidates; i += THREADS) {
+                const uint64_t mine = found.pool[i];
+                const int place = mine != 0 ? place_of(mine, candidates) : top;
+                if (place < top) {
+                    top_ids[(long long)row * top + place] = (int)~(uint32_t)mine;
+                    top_logprobs[(long long)row * top + place] = (key_value((uint32_t)(mine >> 32)) - s.m) - log_s;
+                }
+            }
     }
 }
 
@@ -444,13 +481,20 @@ int launch(const void* logits, long long ld, const int* targets, float* logprob,
     cfg.blockDim = dim3(THREADS);
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = cluster;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    int n = 0;
+    if (cluster > 1) {
+        attr[n].id = cudaLaunchAttributeClusterDimension;
+        attr[n].val.clusterDim.x = cluster;
+        attr[n].val.clusterDim.y = attr[n].val.clusterDim.z = 1;
+        ++n;
+    }
+    if (lp_pdl_enabled()) {
+        attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[n].val.programmaticStreamSerializationAllowed = 1;
+        ++n;
+    }
     cfg.attrs = attr;
-    cfg.numAttrs = lp_pdl_enabled() ? 2 : 1;
+    cfg.numAttrs = n;
     cudaLaunchKernelEx(&cfg, top ? token_logprobs_kernel<T, true> : token_logprobs_kernel<T, false>, (const T*)logits, ld, targets, logprob, entropy,
                        rank, top_ids, top_logprobs, V, top, cluster);
     return lp_check_launch("token_logprobs");

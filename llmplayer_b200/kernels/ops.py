@@ -417,9 +417,9 @@ def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
 
 def _on_current_device(what: str, *tensors: Optional[torch.Tensor]) -> None:
     """All on the device whose stream the launch goes to."""
-    device = torch.cuda.current_device()
+    device = torch._C._cuda_getDevice()
     for t in tensors:
-        if t is not None and t.device.index != device:
+        if t is not None and t.get_device() != device:
             raise KernelError(f"{what}: a tensor on {t.device}, the current device is cuda:{device}")
 
 
