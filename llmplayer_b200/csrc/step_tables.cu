@@ -1,5 +1,5 @@
-// What a batch of sequences that continue one prompt needs beside its products: a step's tables built from the sequences'
-// lengths, pages of the cache copied for new forks, and attention over pages that all sequences share.
+// What a batch of sequences that continue one prompt needs of its cache: a step's tables built from the sequences' lengths, and
+// pages copied for new forks.
 #include "common.cuh"
 
 namespace {
@@ -72,46 +72,6 @@ copy_pages_kernel(uint4* __restrict__ storage, long long run_stride, int page_ve
     for (int i = blockIdx.x * blockDim.x + threadIdx.x; i < page_vectors; i += gridDim.x * blockDim.x) dst[i] = src[i];
 }
 
-// ============================================================================ attention
-// One warp per query token and head: keys 32 at a time, a lane per key for the scores, a lane per features for the values.
-__global__ void __launch_bounds__(128)
-attention_shared_kernel(const __nv_bfloat16* __restrict__ q, __nv_bfloat16* __restrict__ out, const __nv_bfloat16* __restrict__ pages,
-                        const int* __restrict__ table, int width, const int* __restrict__ q_start, const int* __restrict__ kv_len, int B, int T,
-                        int H, int G, int hd, int shared_pages, float scale_log2) {
-    lp_grid_wait();
-    lp_grid_release();
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int at = blockIdx.x * 4 + warp;
-    const int t = at / H, h = at % H, g = h / (H / G);
-    if (t >= T) return;
-    int b = 0;
-    while (b < B && q_start[b + 1] <= t) ++b;
-    if (b >= B) return;                                      // behind the last sequence
-    const int pos = kv_len[b] - (q_start[b + 1] - t);
-    const __nv_bfloat16* query = q + ((long long)t * H + h) * hd;
-    float m = -INFINITY, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int k0 = 0; k0 <= pos; k0 += 32) {
-        const int block = k0 >> 6;
-        const int page = table[(long long)(block < shared_pages ? 0 : b) * width + block];
-        const __nv_bfloat16* k = pages + (((long long)page * 2 * G + g) * 64 + (k0 & 63)) * hd;
-        const __nv_bfloat16* v = k + (long long)G * 64 * hd;
-        float s = 0.f;
-        for (int d = 0; d < hd; ++d) s += __bfloat162float(query[d]) * __bfloat162float(k[lane * hd + d]);
-        s = k0 + lane <= pos ? s * scale_log2 : -INFINITY;
-        const float mn = fmaxf(m, lp_warp_max(s));
-        const float f = exp2f(m - mn), e = exp2f(s - mn);
-        m = mn;
-        l = l * f + lp_warp_sum(e);
-        for (int u = 0; u < hd / 32; ++u) o[u] *= f;
-        for (int j = 0; j < 32 && k0 + j <= pos; ++j) {
-            const float w = __shfl_sync(0xffffffffu, e, j);
-            for (int u = 0; u < hd / 32; ++u) o[u] += w * __bfloat162float(v[j * hd + u * 32 + lane]);
-        }
-    }
-    for (int u = 0; u < hd / 32; ++u)
-        out[((long long)t * H + h) * hd + u * 32 + lane] = __float2bfloat16_rn(l > 0.f ? o[u] / l : 0.f);
-}
-
 }  // namespace
 
 // first, count int32 [B]; shared [num_shared], own [num_own] page numbers; table [B, width]; the others may be null, together:
@@ -139,15 +99,4 @@ extern "C" int lp_copy_pages(void* storage, int runs, long long num_pages, long 
     const int vectors = (int)(page_bytes / 16);
     lp_launch(copy_pages_kernel, dim3((vectors + 1023) / 1024, n, runs), dim3(256), 0, stream, (uint4*)storage, num_pages * (page_bytes / 16), vectors, pairs);
     return lp_check_launch("copy_pages");
-}
-
-// q, out: bf16 [T, H, hd]; pages bf16 [num_pages, 2, G, 64, hd]; table int32 [B, width], whose first shared_pages columns are
-// the same in every row; q_start int32 [B + 1]; kv_len int32 [B], lengths with the new tokens.
-extern "C" int lp_attention_shared(const void* q, void* out, const void* pages, const int* table, int width, const int* q_start, const int* kv_len,
-                                   int B, int T, int H, int G, int hd, int shared_pages, float scale, cudaStream_t stream) {
-    if (B <= 0 || T <= 0 || G <= 0 || H % G || (hd != 64 && hd != 128) || shared_pages < 0 || shared_pages > width)
-        LP_REFUSE("attention_shared: %d sequences, %d tokens, %d heads on %d of %d, %d shared pages", B, T, H, G, hd, shared_pages);
-    lp_launch(attention_shared_kernel, dim3((T * H + 3) / 4), dim3(128), 0, stream, (const __nv_bfloat16*)q, (__nv_bfloat16*)out,
-              (const __nv_bfloat16*)pages, table, width, q_start, kv_len, B, T, H, G, hd, shared_pages, scale * 1.4426950408889634f);
-    return lp_check_launch("attention_shared");
 }

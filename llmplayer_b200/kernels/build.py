@@ -42,7 +42,8 @@ LIBRARIES: Dict[str, str] = {
     "recurrent_step": "recurrent_step.cu",
     "stream_bundle": "stream_bundle.cu",
     "scoring": "scoring.cu",
-    "shared_prefix": "shared_prefix.cu",
+    "step_tables": "step_tables.cu",
+    "attention_shared": "attention_shared.cu",
 }
 HEADERS = ("common.cuh", "attention_noalloc.h", "tcgen05_utils.cuh", "attention_decode.cuh", "bf16_parts.cuh")
 

@@ -141,11 +141,13 @@ _SIGNATURES = {
     "scoring": {
         "lp_token_logprobs": [_P, _I, ctypes.c_longlong, _P, _P, _P, _P, _P, _P, _I, _I, _I, _P],
     },
-    "shared_prefix": {
+    "step_tables": {
         "lp_step_tables": [_P, _P, _P, _I, _P, _I, _P, _P, _P, _P, _I, _P, _I, _I, _I, _P],
         "lp_copy_pages_most": [],
         "lp_copy_pages": [_P, _I, ctypes.c_longlong, ctypes.c_longlong, _P, _P, _I, _P],
-        "lp_attention_shared": [_P, _P, _P, _P, _I, _P, _P, _I, _I, _I, _I, _I, _I, _F, _P],
+    },
+    "attention_shared": {
+        "lp_attention_shared": [_P, _P, _P, ctypes.c_longlong, _P, _I, _P, _P, _I, _I, _I, _I, _I, _I, _I, _F, _I, _P, _P, _P, _P],
     },
 }
 
@@ -769,7 +771,8 @@ def check_kernel_status() -> None:
         raise KernelError(f"a tensor-core kernel gave up waiting on a barrier (code {code}: "
                           "1 = loader, 2 = MMA issuer, 3 = epilogue, 4-5 = operand maker; 2x the same in the "
                           "persistent product, 5x in the experts' (55: more choices than announced); "
-                          "6 = a page of the decode attention; 61 = a record of the chunked recurrence; 62 = rows of the latent attention; 7x = the float32 product)")
+                          "6 = a page of the decode attention; 61 = a record of the chunked recurrence; 62 = rows of the latent attention; 7x = the float32 product; "
+                          "8x = attention over shared pages)")
 
 
 def _token_tile(tokens: int, gated: bool) -> int:
@@ -1281,8 +1284,8 @@ def attention_shared(q: torch.Tensor, out: torch.Tensor, pages: torch.Tensor, pa
 
     ``q``, ``out``: bfloat16 [T, H * hd], the new tokens of the sequences one behind the other; ``q_start`` int32 [B + 1]: where
     each sequence's begin (a sequence may have none); ``kv_len`` int32 [B]: lengths with the new tokens; ``max_new``: no sequence has
-    more new tokens. A token sees its sequence's keys up to its own position. Rows of ``q`` behind the last sequence are not
-    read, and those of ``out`` stay as they are. ``scratch(name, shape, dtype)`` supplies buffers for partial results."""
+    more new tokens. A token sees its sequence's keys up to its own position. What rows of ``q`` behind the last sequence hold does not
+    matter, and those of ``out`` stay as they are. ``scratch(name, shape, dtype)`` supplies buffers for partial results."""
     what = "attention_shared"
     _check_attention(q, out, pages, page_table, num_heads, num_kv_heads, head_dim, what)
     _want(q_start, f"{what} q_start", torch.int32, 1)
@@ -1300,11 +1303,32 @@ def attention_shared(q: torch.Tensor, out: torch.Tensor, pages: torch.Tensor, pa
         raise KernelError(f"{what}: at most {max_new} new tokens per sequence")
     if T == 0:
         return out
-    lib = library("shared_prefix")
-    _check(lib, lib.lp_attention_shared(q.data_ptr(), out.data_ptr(), pages.data_ptr(), page_table.data_ptr(), page_table.shape[1],
-                                        q_start.data_ptr(), kv_len.data_ptr(), B, T, num_heads, num_kv_heads, head_dim, int(shared_pages),
-                                        float(scale), _stream()))
+    splits, slots = shared_split(T, num_heads, num_kv_heads, int(shared_pages))
+    parts = scratch("shared_partials", (slots * T * num_heads * (head_dim + 2),), torch.float32) if slots else None
+    part_o = _ptr(parts)
+    part_ml = part_o + 4 * slots * T * num_heads * head_dim if slots else None
+    lib = library("attention_shared")
+    _check(lib, lib.lp_attention_shared(q.data_ptr(), out.data_ptr(), pages.data_ptr(), pages.shape[0], page_table.data_ptr(), page_table.shape[1],
+                                        q_start.data_ptr(), kv_len.data_ptr(), B, T, int(max_new), num_heads, num_kv_heads, head_dim, int(shared_pages),
+                                        float(scale), splits, part_o, part_ml, kernel_status().data_ptr(), _stream()))
     return out
+
+
+SHARED_ROWS = 128             # (token, query head) rows of a tile of the shared pages' products
+SHARED_SPLITS_MOST = 32
+
+
+@functools.lru_cache(maxsize=512)
+def shared_split(tokens: int, num_heads: int, num_kv_heads: int, shared_pages: int):
+    """(shares, partial results per row) of the shared pages: a CTA takes two tiles of rows of one key/value head and one share of
+    the blocks of 128 keys. As many shares as make the last round of CTAs end soonest, counting a CTA's start and end as three
+    blocks; a single tile leaves two partial results per share (its CTA's two chains take alternate blocks)."""
+    if shared_pages == 0:
+        return 0, 0
+    tiles = -(-tokens // (SHARED_ROWS // (num_heads // num_kv_heads)))
+    ctas, blocks, sms = -(-tiles // 2) * num_kv_heads, -(-shared_pages // 2), num_sms()
+    best = min(range(1, min(blocks, SHARED_SPLITS_MOST) + 1), key=lambda n: (-(-ctas * n // sms) * (-(-blocks // n) + 3), n))
+    return best, (2 * best if tiles == 1 else best)
 
 
 # --------------------------------------------------------------------------- a step's tables, copies of pages
@@ -1340,7 +1364,7 @@ def step_tables(first: torch.Tensor, count: torch.Tensor, shared: torch.Tensor, 
             raise KernelError(f"{what}: {B} sequences, {q_start.numel()} offsets, {kv_len.numel()} lengths, {tokens} positions of "
                               f"{seq_ids.numel()} tokens")
     _on_current_device(what, first, count, shared, own, page_table, *rest)
-    lib = library("shared_prefix")
+    lib = library("step_tables")
     _check(lib, lib.lp_step_tables(first.data_ptr(), count.data_ptr(), shared.data_ptr(), shared.numel(), own.data_ptr(), own.numel(),
                                    _ptr(q_start), _ptr(kv_len), _ptr(positions), _ptr(seq_ids), tokens, page_table.data_ptr(),
                                    page_table.shape[1], B, int(page_size), _stream()))
@@ -1368,7 +1392,7 @@ def copy_pages(storage: torch.Tensor, sources, targets) -> None:
         return
     if page_bytes % 16 or storage.data_ptr() % 16:
         raise KernelError(f"{what}: pages of {page_bytes} bytes at {storage.data_ptr():#x}: they must be whole vectors of 16 bytes")
-    lib = library("shared_prefix")
+    lib = library("step_tables")
     most = lib.lp_copy_pages_most()
     for a in range(0, len(targets), most):
         n = min(most, len(targets) - a)
