@@ -19,30 +19,28 @@
 namespace {
 
 constexpr int ROWS = 128;                 // rows of a product: (token, query head) pairs of one key/value head
-constexpr int KEYS = 2 * PAGE;            // keys per block
-constexpr int THREADS = 640;              // warp 0: loader, warp 1: MMA (2 and 3: nothing), warps 4-11 and 12-19: the softmax of the two chains
-// Registers are granted 96 to a thread at launch (61,440 in all) and shared out again between the warpgroups.
-constexpr int REGS_FEW = 64, REGS_MANY = 104;
-static_assert(128 * REGS_FEW + 512 * REGS_MANY <= THREADS * 96, "");
+constexpr int THREADS = 384;              // warp 0: loader, warp 1: MMA (2 and 3: nothing), warps 4-7 and 8-11: the softmax of the two chains
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float RESCALE_ABOVE = 8.0f;     // log2: how far a row's reference maximum may lag behind its maximum (a factor of 256)
 
 // ============================================================================ the shared pages
-// A CTA has two chains of products and softmaxes that take turns on the tensor cores and the exponential units: while one chain's
-// scores are turned into weights, the other's products run. With two tiles of rows each chain has one, and both read each
-// block of keys from the same stage; with a single tile the chains share it and take alternate blocks (their results are two
-// partial ones). Per block and chain:
-//   S[128 x 128] = Q K^T (tensor memory)  ->  two threads per row, each with half of the keys: maximum (joined in shared memory),
-//   exp2, sum, weights as bfloat16 over S in tensor memory
+// A CTA has two chains of products and softmaxes, so that the tensor cores and the exponential units are both busy. With two tiles of
+// rows each chain has one, and both read each page from the same stage; with a single tile the chains share it and take
+// alternate pages (their results are two partial ones). Per page and chain:
+//   S[128 x 64] = Q K^T (tensor memory)  ->  a thread per row: maximum, exp2, sum, weights as bfloat16 over S in tensor memory
 //   ->  O[128 x HD] += P V (P from tensor memory, V from shared memory, contiguous in N).
+// A chain has two S tiles: the scores of its next page are there when it has finished with one, so a chain never waits for
+// the tensor cores. (With one tile of 128 keys per chain it did, and the two chains' softmaxes ran one behind the other: 4,000 cycles per
+// 128 keys at heads of 128, 2,370 us for 40 x 190 tokens over 500 shared pages, 32 heads on 8.)
 template <int HD> struct Shape {
     static constexpr int BLOCKS = HD / 64;                          // blocks of 64 features (one swizzle row each)
-    static constexpr int TILE = KEYS * HD * 2;                      // keys or values of a block
+    static constexpr int TILE = PAGE * HD * 2;                      // keys or values of a page
     static constexpr int Q_TILE = ROWS * HD * 2;
-    static constexpr int SLOTS = HD == 64 ? 8 : 5;                  // K0 V0 K1 V1 ...
-    static constexpr int SMEM = 2 * Q_TILE + SLOTS * TILE + 1024 /* alignment */ + 256 /* barriers */ + 2 * ROWS * 4 /* positions, then maxima */;
-    static_assert(SMEM <= 227 * 1024 && ROWS == KEYS, "");
-    static constexpr int S_COL = 0, O_COL = 256;                    // chain c: S at 128 c, O at 256 + HD c
+    static constexpr int SLOTS = HD == 64 ? 16 : 10;
+    static constexpr int SMEM = 2 * Q_TILE + SLOTS * TILE + 1024 /* alignment */ + 512 /* barriers */ + 2 * ROWS * 4 /* positions */;
+    static constexpr int OUT_ROW = HD * 4 + 16;                     // a row of results on its way out: where the ring was
+    static_assert(SMEM <= 227 * 1024 && 2 * ROWS * OUT_ROW <= SLOTS * TILE, "");
+    static constexpr int S_COL = 0, O_COL = 256;                    // chain c: S at 128 c and 128 c + 64, O at 256 + HD c
     static constexpr int TMEM_COLS = 512;
 };
 
@@ -94,13 +92,6 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* r) {
           "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
         : "memory");
 }
-__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
-        ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
-          "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
-        : "memory");
-}
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 // Two float32 operations in one instruction (Blackwell's packed forms).
 __device__ __forceinline__ void fma2(float& x0, float& x1, float a, float b) {            // x = x * a + b
@@ -124,13 +115,6 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     return d;
 }
 
-// A float as an integer of the same order (its own inverse; no number becomes the largest or the smallest).
-__device__ __forceinline__ int ordered(float x) {
-    const int b = __float_as_int(x);
-    return b ^ ((b >> 31) & 0x7fffffff);
-}
-__device__ __forceinline__ float unordered(int k) { return __int_as_float(k ^ ((k >> 31) & 0x7fffffff)); }
-
 struct SharedArgs {
     const int* table;            // the first row of the page table: its first `pages` entries are the shared pages
     const int* q_start;          // [B + 1]
@@ -142,7 +126,7 @@ struct SharedArgs {
     int* status;
 };
 
-// grid: (splits x pairs of row tiles, G); a split takes consecutive blocks of keys.
+// grid: (splits x pairs of row tiles, G); a split takes consecutive pages.
 template <int HD>
 __global__ void __launch_bounds__(THREADS, 1)
 attention_shared_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_kv, const SharedArgs a) {
@@ -155,30 +139,36 @@ attention_shared_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
     uint64_t* full = (uint64_t*)(ring + SLOTS * TILE);             // [SLOTS]
     uint64_t* empty = full + SLOTS;                                // [SLOTS]
     uint64_t* q_full = empty + SLOTS;
-    uint64_t* s_ready = q_full + 1;                                // [2] scores of a chain are in tensor memory
-    uint64_t* p_ready = s_ready + 2;                               // [2] its weights are
-    uint64_t* o_ready = p_ready + 2;                               // [2] weights times values have been added
+    uint64_t* s_ready = q_full + 1;                                // [chain][tile] scores are in tensor memory
+    uint64_t* p_ready = s_ready + 4;                               // [chain][tile] weights are
+    uint64_t* o_ready = p_ready + 4;                               // [chain] weights times values have been added
     uint32_t* tmem_slot = (uint32_t*)(o_ready + 2);
-    int* position = (int*)((uint8_t*)full + 256);                  // [2 ROWS]: of the CTA's tokens, -1: nobody's
+    int* position = (int*)((uint8_t*)full + 512);                  // [2 ROWS]: of the CTA's tokens, -1: nobody's
+    static_assert((2 * SLOTS + 11) * 8 + 4 <= 512, "");
 
     const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;       // alike in all lanes
     const int per_tile = ROWS / a.R, tiles = (a.T + per_tile - 1) / per_tile;
     const int pair = blockIdx.x / a.splits, split = blockIdx.x - pair * a.splits, g = blockIdx.y;
-    const bool alone = tiles == 1;                                 // one tile of rows: the chains take alternate blocks
+    const bool alone = tiles == 1;                                 // one tile of rows: the chains take alternate pages
     const int chains = alone || pair * 2 + 1 < tiles ? 2 : 1;
     const int t0 = pair * 2 * per_tile;
-    const int all_blocks = (a.pages + 1) / 2;
-    const int first = (int)((long long)all_blocks * split / a.splits), end = (int)((long long)all_blocks * (split + 1) / a.splits);
-    const int blocks = end - first;
-    // chain c takes block i
-    auto takes = [&](int i, int c) { return i < blocks && (alone ? (i & 1) == c : c < chains); };
+    const int first = (int)((long long)a.pages * split / a.splits), n = (int)((long long)a.pages * (split + 1) / a.splits) - first;
+    // A chain's k-th page is page k of the share, or every second one. Tiles are asked for in the order in which the products take
+    // them: `lead` pages' keys, then the values of a page and the keys of the page `lead` behind it.
+    const int step = alone ? 2 : 1, lead = 2 * step;
+    auto page_of = [&](int k, int c) { return alone ? 2 * k + c : k; };
+    auto turns = [&](int c) { return alone ? (n + 1 - c) / 2 : c < chains ? n : 0; };
+    auto keys_at = [&](int i) { return i < lead ? i : 2 * i - lead + 1; };
+    auto values_at = [&](int i) { return min(n, lead + i) + i; };
 
     if (threadIdx.x == 0) {
         asm volatile("prefetch.tensormap [%0];" ::"l"(&map_q) : "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(&map_kv) : "memory");
         mbar_init(q_full, 1);
         for (int s = 0; s < SLOTS; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
-        for (int c = 0; c < 2; ++c) { mbar_init(&s_ready[c], 1); mbar_init(&p_ready[c], 8); mbar_init(&o_ready[c], 1); }
+        for (int i = 0; i < 4; ++i) { mbar_init(&s_ready[i], 1); mbar_init(&p_ready[i], 4); }
+        mbar_init(&o_ready[0], 1);
+        mbar_init(&o_ready[1], 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 1) {
@@ -192,7 +182,6 @@ attention_shared_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
     lp_grid_wait();
     lp_grid_release();             // behind the wait: what the kernel for the own pages reads early is then there
 
-    if (warp < 4) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS_FEW));
     if (warp == 0) {
         // ------------------------------------------------------------ loader
         if (lane == 0) {
@@ -204,165 +193,149 @@ attention_shared_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
                 for (int f = 0; f < SH::BLOCKS; ++f)
                     tma_load_3d(q_tiles + c * SH::Q_TILE + f * (ROWS * 128), &map_q, f * 64, g * a.R, t0 + c * per_tile, q_full);
         }
-        // The lanes hold the next 32 page numbers, so that a request does not begin with a round trip to memory.
-        int held = 0;
+        // The lanes hold page numbers (lane j those of pages j, j + 32, ... of the share, the last two of them), so that a request does not
+        // begin with a round trip to memory.
+        int held = lane < n ? a.table[first + lane] : 0, before = 0;
+        int loaded = 32;
         bool ok = true;
-        for (int i = 0; i < blocks && ok; ++i) {
-            const int page0 = (first + i) * 2, count = min(2, a.pages - page0);
-            if ((i & 15) == 0) held = page0 + lane < a.pages ? a.table[page0 + lane] : 0;
-            const int page_a = __shfl_sync(0xffffffffu, held, (2 * i) & 31), page_b = __shfl_sync(0xffffffffu, held, (2 * i + 1) & 31);
-            for (int which = 0; which < 2 && ok; ++which) {         // the keys of a block, then its values
-                const int n = 2 * i + which, s = n % SLOTS;
-                ok = __all_sync(0xffffffffu, mbar_wait(&empty[s], ((n / SLOTS) & 1) ^ 1));
-                if (lane == 0) {
-                    if (!ok) { atomicExch(a.status, 81); break; }
-                    mbar_expect_tx(&full[s], (uint32_t)(count * PAGE * HD * 2));
-#pragma unroll
-                    for (int k = 0; k < 2; ++k) {
-                        const int row = (((k ? page_b : page_a) * 2 + which) * a.G + g) * PAGE;
-                        if (k < count)
-#pragma unroll
-                            for (int f = 0; f < SH::BLOCKS; ++f)
-                                tma_load_2d(ring + s * TILE + f * (KEYS * 128) + k * (PAGE * 128), &map_kv, f * 64, row, &full[s]);
-                    }
-                }
+        int at = 0;
+        auto request = [&](int i, int which) {
+            if (i >= loaded) {                                     // keys run ahead of values by less than 32 pages
+                before = held;
+                held = loaded + lane < n ? a.table[first + loaded + lane] : 0;
+                loaded += 32;
             }
+            const int page = __shfl_sync(0xffffffffu, i >= loaded - 32 ? held : before, i & 31);
+            const int s = at % SLOTS;
+            ok = __all_sync(0xffffffffu, mbar_wait(&empty[s], ((at / SLOTS) & 1) ^ 1));
+            if (!ok) { if (lane == 0) atomicExch(a.status, 81); return; }
+            if (lane == 0) {
+                mbar_expect_tx(&full[s], (uint32_t)TILE);
+                const int row = ((page * 2 + which) * a.G + g) * PAGE;
+#pragma unroll
+                for (int f = 0; f < SH::BLOCKS; ++f) tma_load_2d(ring + s * TILE + f * (PAGE * 128), &map_kv, f * 64, row, &full[s]);
+            }
+            ++at;
+        };
+        for (int i = 0; i < min(lead, n) && ok; ++i) request(i, 0);
+        for (int i = 0; i < n && ok; ++i) {
+            request(i, 1);
+            if (ok && i + lead < n) request(i + lead, 0);
         }
+        if (!ok)                                                   // the copies in flight land before the CTA ends
+            for (int i = max(0, at - SLOTS); i < at; ++i) mbar_wait(&full[i % SLOTS], (i / SLOTS) & 1);
         __syncwarp();
     } else if (warp == 1) {
         // ------------------------------------------------------------ MMA issuer
         constexpr uint32_t base_idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(ROWS >> 4) << 24);
+        constexpr uint32_t idesc_s = base_idesc | ((uint32_t)(PAGE >> 3) << 17);
         constexpr uint32_t idesc_pv = base_idesc | (1u << 16) | ((uint32_t)(HD >> 3) << 17);                  // V: contiguous in N
         const uint32_t leader = elect_one();
-        const uint64_t desc_q = smem_desc(smem_u32(q_tiles)), desc_k = smem_desc(smem_u32(ring)), desc_v = smem_desc_mn(smem_u32(ring), KEYS * 128);
-        bool ok = __all_sync(0xffffffffu, mbar_wait(q_full, 0));
-        if (!ok && leader) atomicExch(a.status, 82);
-        uint32_t turn[2] = {0, 0};                             // blocks of each chain whose weights were awaited
-        auto last_chain = [&](int i, int c) { return c == 1 || !takes(i, 1); };
+        const uint64_t desc_q = smem_desc(smem_u32(q_tiles)), desc_k = smem_desc(smem_u32(ring)), desc_v = smem_desc_mn(smem_u32(ring), PAGE * 128);
         auto arrived = [&](uint64_t* bar, uint32_t parity, int code) {
             const bool yes = __all_sync(0xffffffffu, mbar_wait(bar, parity));
             if (!yes && leader) atomicExch(a.status, code);
             return yes;
         };
-        auto scores = [&](int i, int c) -> bool {
-            const int n = 2 * i, s = n % SLOTS;
-            if (!arrived(&full[s], (n / SLOTS) & 1, 83)) return false;
+        bool ok = arrived(q_full, 0, 82);
+        const int turns_of[2] = {turns(0), turns(1)};
+        // the last chain that takes a tile gives its slot back
+        auto last_chain = [&](int c) { return alone || c == chains - 1; };
+        auto scores = [&](int k, int c) -> bool {
+            const int at = keys_at(page_of(k, c)), s = at % SLOTS;
+            if (!arrived(&full[s], (at / SLOTS) & 1, 83)) return false;
             tcgen05_fence_after();
             const uint64_t dq = desc_q + (uint64_t)((alone ? 0 : c) * (SH::Q_TILE >> 4)), dk = desc_k + (uint64_t)(s * (TILE >> 4));
-            const uint32_t idesc = base_idesc | ((uint32_t)(min(2, a.pages - (first + i) * 2) * PAGE >> 3) << 17);
 #pragma unroll
-            for (int k = 0; k < HD / 16; ++k)                  // 16 features per instruction; 4 instructions per block of 64
-                mma_ss(leader, tmem_base + SH::S_COL + c * KEYS, dq + (uint64_t)((k >> 2) * (ROWS * 128 >> 4) + (k & 3) * 2),
-                       dk + (uint64_t)((k >> 2) * (KEYS * 128 >> 4) + (k & 3) * 2), idesc, k > 0 ? 1u : 0u);
-            commit(leader, &s_ready[c]);
-            if (last_chain(i, c)) commit(leader, &empty[s]);
+            for (int j = 0; j < HD / 16; ++j)                  // 16 features per instruction; 4 instructions per block of 64
+                mma_ss(leader, tmem_base + SH::S_COL + c * 128 + (k & 1) * PAGE, dq + (uint64_t)((j >> 2) * (ROWS * 128 >> 4) + (j & 3) * 2),
+                       dk + (uint64_t)((j >> 2) * (PAGE * 128 >> 4) + (j & 3) * 2), idesc_s, j > 0 ? 1u : 0u);
+            commit(leader, &s_ready[c * 2 + (k & 1)]);
+            if (last_chain(c)) commit(leader, &empty[s]);
             return true;
         };
-        auto values = [&](int i, int c) -> bool {
-            const int n = 2 * i + 1, s = n % SLOTS;
-            if (!arrived(&p_ready[c], turn[c] & 1, 84) || !arrived(&full[s], (n / SLOTS) & 1, 83)) return false;
+        auto values = [&](int k, int c) -> bool {
+            const int at = values_at(page_of(k, c)), s = at % SLOTS;
+            if (!arrived(&full[s], (at / SLOTS) & 1, 83) || !arrived(&p_ready[c * 2 + (k & 1)], (k >> 1) & 1, 84)) return false;
             tcgen05_fence_after();
             const uint64_t dv = desc_v + (uint64_t)(s * (TILE >> 4));
-            const uint32_t d = tmem_base + SH::O_COL + c * HD, p = tmem_base + SH::S_COL + c * KEYS;
-            mma_ts(leader, d, p, dv, idesc_pv, turn[c] > 0 ? 1u : 0u);
+            const uint32_t d = tmem_base + SH::O_COL + c * HD, p = tmem_base + SH::S_COL + c * 128 + (k & 1) * PAGE;
+            mma_ts(leader, d, p, dv, idesc_pv, k > 0 ? 1u : 0u);
 #pragma unroll
-            for (int k = 1; k < PAGE / 16; ++k) mma_ts(leader, d, p + k * 8, dv + (uint64_t)(k * (2048 >> 4)), idesc_pv, 1u);
-            if ((first + i) * 2 + 1 < a.pages)                 // the block's second page
-#pragma unroll
-                for (int k = PAGE / 16; k < KEYS / 16; ++k) mma_ts(leader, d, p + k * 8, dv + (uint64_t)(k * (2048 >> 4)), idesc_pv, 1u);
-            ++turn[c];
+            for (int j = 1; j < PAGE / 16; ++j) mma_ts(leader, d, p + j * 8, dv + (uint64_t)(j * (2048 >> 4)), idesc_pv, 1u);
             commit(leader, &o_ready[c]);
-            if (last_chain(i, c)) commit(leader, &empty[s]);
+            if (last_chain(c)) commit(leader, &empty[s]);
             return true;
         };
-        // A chain's next scores go over its weights, which the products issued before them have read.
-        const int ahead = alone ? 2 : 1;
-        for (int i = 0; i < ahead; ++i)
+        // A chain's scores go over the weights of two pages before, which the products issued before them have read.
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
 #pragma unroll
             for (int c = 0; c < 2; ++c)
-                if (ok && takes(i, c)) ok = scores(i, c);
-        for (int i = 0; i < blocks && ok; ++i)
+                if (ok && k < turns_of[c]) ok = scores(k, c);
+        for (int k = 0; k < turns_of[0] && ok; ++k)            // chain 0 has as many turns as chain 1, or one more
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-                if (ok && takes(i, c)) ok = values(i, c);
-                if (ok && takes(i, c) && takes(i + ahead, c)) ok = scores(i + ahead, c);
+                if (ok && k < turns_of[c]) ok = values(k, c);
+                if (ok && k + 2 < turns_of[c]) ok = scores(k + 2, c);
             }
         __syncwarp();
     } else if (warp >= 4) {
-        // ------------------------------------------------------------ softmax: two threads per row
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS_MANY));
-        constexpr int HALF = KEYS / 2, OHALF = HD / 2;
-        const int c = (warp - 4) >> 3, half = ((warp - 4) >> 2) & 1, quarter = warp & 3, r = quarter * 32 + lane;
+        // ------------------------------------------------------------ softmax: a thread per row
+        const int c = (warp - 4) >> 2, quarter = warp & 3, r = quarter * 32 + lane;
         // the positions of the CTA's tokens: a token that itself lies among the shared pages sees them up to its own
-        for (int i = threadIdx.x - 128; i < 2 * per_tile; i += 512) position[i] = -1;
-        asm volatile("bar.sync 1, 512;" ::: "memory");
-        for (int b = threadIdx.x - 128; b < a.B; b += 512) {
+        for (int i = threadIdx.x - 128; i < 2 * per_tile; i += 256) position[i] = -1;
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+        for (int b = threadIdx.x - 128; b < a.B; b += 256) {
             const int from = a.q_start[b], to = a.q_start[b + 1], len = a.kv_len[b];
             for (int t = max(from, t0); t < min(to, t0 + 2 * per_tile); ++t) position[t - t0] = len - (to - t);
         }
-        asm volatile("bar.sync 1, 512;" ::: "memory");
+        asm volatile("bar.sync 1, 256;" ::: "memory");
         const int token = t0 + (alone ? 0 : c) * per_tile + r / a.R, head = g * a.R + r % a.R;
         const bool real = r < per_tile * a.R && token < a.T && c < chains;
         const int seen = real ? min(position[token - t0] + 1, a.pages * PAGE) : 0;      // shared keys that the row sees
         const float scale = a.scale_log2;
-        const uint32_t lane_addr = tmem_base + ((uint32_t)(quarter * 32) << 16);
-        const uint32_t s_addr = lane_addr + SH::S_COL + c * KEYS, o_addr = lane_addr + SH::O_COL + c * HD + half * OHALF;
-        // the rows' maxima so far, as integers of the same order; where the positions were
-        asm volatile("bar.sync 1, 512;" ::: "memory");
-        int* most_of_row = position + c * ROWS + r;
-        if (half == 0) *most_of_row = ordered(-INFINITY);
-        const int pair_barrier = 2 + c * 4 + quarter;                 // the two warps of 32 rows
-        asm volatile("bar.sync %0, 64;" ::"r"(pair_barrier) : "memory");
+        const uint32_t lane_addr = tmem_base + ((uint32_t)(quarter * 32) << 16), o_addr = lane_addr + SH::O_COL + c * HD;
+        const int count = turns(c);
         float m = NEG_BIG, l = 0.f;
-        uint32_t turn = 0;
         bool ok = true;
-        for (int i = 0; i < blocks; ++i) {
-            if (!takes(i, c)) continue;
-            // after a wait that ran out the warp goes on without tensor memory: its partner counts on it at the barriers
-            if (ok && !__all_sync(0xffffffffu, mbar_wait(&s_ready[c], turn & 1))) { if (lane == 0) atomicExch(a.status, 85); ok = false; }
+        for (int k = 0; k < count; ++k) {
+            const uint32_t s_addr = lane_addr + SH::S_COL + c * 128 + (k & 1) * PAGE;
+            ok = __all_sync(0xffffffffu, mbar_wait(&s_ready[c * 2 + (k & 1)], (k >> 1) & 1));
+            if (!ok) { if (lane == 0) atomicExch(a.status, 85); break; }
             tcgen05_fence_after();
-            uint32_t s[HALF];
-            if (ok) {
-                tmem_ld32(s_addr + half * HALF, s);
-                tmem_ld32(s_addr + half * HALF + 32, s + 32);
-                tmem_ld_wait();
-            } else {
+            uint32_t s[PAGE];
+            tmem_ld32(s_addr, s);
+            tmem_ld32(s_addr + 32, s + 32);
+            tmem_ld_wait();
+            const int key0 = (first + page_of(k, c)) * PAGE;
+            if (__any_sync(0xffffffffu, seen < key0 + PAGE)) {
 #pragma unroll
-                for (int j = 0; j < HALF; ++j) s[j] = 0;
-            }
-            const int key0 = (first + i) * KEYS + half * HALF;
-            if (__any_sync(0xffffffffu, seen < key0 + HALF)) {
-#pragma unroll
-                for (int j = 0; j < HALF; ++j)
+                for (int j = 0; j < PAGE; ++j)
                     if (key0 + j >= seen) s[j] = 0xff800000u;
             }
             float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-            for (int j = 0; j < HALF; j += 8)
+            for (int j = 0; j < PAGE; j += 8)
 #pragma unroll
-                for (int k = 0; k < 4; ++k) mx4[k] = max3(mx4[k], __uint_as_float(s[j + 2 * k]), __uint_as_float(s[j + 2 * k + 1]));
-            // The other thread of the row adds its maximum; nobody gets to the next block before both have read (p_ready). Behind
-            // the barrier the scores have been read by both, too, and the weights may go over them.
-            atomicMax(most_of_row, ordered(fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]))));
-            asm volatile("bar.sync %0, 64;" ::"r"(pair_barrier) : "memory");
-            const float mx = unordered(*(volatile int*)most_of_row) * scale;
+                for (int u = 0; u < 4; ++u) mx4[u] = max3(mx4[u], __uint_as_float(s[j + 2 * u]), __uint_as_float(s[j + 2 * u + 1]));
+            const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * scale;
             // The reference follows only when the row's maximum has outgrown it by more than RESCALE_ABOVE; then the output so far comes
             // down to it, which must have been added up before and waits for nothing else (the next product follows p_ready).
             const bool moves = mx > m + RESCALE_ABOVE;
-            if (__any_sync(0xffffffffu, moves) && turn > 0) {
-                if (ok && !__all_sync(0xffffffffu, mbar_wait(&o_ready[c], (turn - 1) & 1))) { if (lane == 0) atomicExch(a.status, 86); ok = false; }
+            if (__any_sync(0xffffffffu, moves) && k > 0) {
+                ok = __all_sync(0xffffffffu, mbar_wait(&o_ready[c], (k - 1) & 1));
+                if (!ok) { if (lane == 0) atomicExch(a.status, 86); break; }
                 tcgen05_fence_after();
                 const float factor = moves ? fast_exp2(m - mx) : 1.0f;
-                if (ok) {
 #pragma unroll
-                    for (int d = 0; d < OHALF; d += 16) {
-                        uint32_t o[16];
-                        tmem_ld16(o_addr + d, o);
-                        tmem_ld_wait();
+                for (int d = 0; d < HD; d += 32) {
+                    uint32_t o[32];
+                    tmem_ld32(o_addr + d, o);
+                    tmem_ld_wait();
 #pragma unroll
-                        for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * factor);
-                        tmem_st16(o_addr + d, o);
-                    }
+                    for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * factor);
+                    tmem_st32(o_addr + d, o);
                 }
             }
             if (moves) {
@@ -370,9 +343,9 @@ attention_shared_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
                 m = mx;
             }
             float sum4[4] = {0.f, 0.f, 0.f, 0.f};
-            uint32_t p[HALF / 2];
+            uint32_t p[PAGE / 2];
 #pragma unroll
-            for (int j = 0; j < HALF / 2; ++j) {
+            for (int j = 0; j < PAGE / 2; ++j) {
                 float e0 = __uint_as_float(s[2 * j]), e1 = __uint_as_float(s[2 * j + 1]);
                 fma2(e0, e1, scale, -m);
                 e0 = fast_exp2(e0);
@@ -380,38 +353,39 @@ attention_shared_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
                 add2(sum4[(j & 1) * 2], sum4[(j & 1) * 2 + 1], e0, e1);
                 p[j] = pack_bf16(e0, e1);
             }
-            if (ok) {
-                tmem_st32(s_addr + half * (HALF / 2), p);
-                tmem_st_wait();
-            }
+            tmem_st32(s_addr, p);
+            tmem_st_wait();
             l += (sum4[0] + sum4[1]) + (sum4[2] + sum4[3]);
             tcgen05_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&p_ready[c]);
-            ++turn;
+            if (lane == 0) mbar_arrive(&p_ready[c * 2 + (k & 1)]);
         }
-        if (turn > 0 && ok && !__all_sync(0xffffffffu, mbar_wait(&o_ready[c], (turn - 1) & 1))) { if (lane == 0) atomicExch(a.status, 86); ok = false; }
+        // The last scores say that all products but two have been added: those two are awaited one by one, as a parity tells only a
+        // phase from the one before it.
+        for (int k = max(0, count - 2); k < count; ++k)
+            if (ok && !__all_sync(0xffffffffu, mbar_wait(&o_ready[c], k & 1))) { if (lane == 0) atomicExch(a.status, 86); ok = false; }
         tcgen05_fence_after();
-        // the two threads of a row add their sums
-        if (half == 1) *most_of_row = __float_as_int(turn > 0 && ok ? l : 0.f);
-        asm volatile("bar.sync %0, 64;" ::"r"(pair_barrier) : "memory");
         const int slot = alone ? split * 2 + c : split;
         const long long row = ((long long)slot * a.T + token) * a.H + head;
-        if (real && half == 0) {
-            a.part_ml[row * 2] = turn > 0 ? m : NEG_BIG;
-            a.part_ml[row * 2 + 1] = turn > 0 && ok ? l + __int_as_float(*most_of_row) : 0.f;
-        }
-        if (turn > 0 && ok) {
+        if (real) *reinterpret_cast<float2*>(a.part_ml + row * 2) = make_float2(count > 0 ? m : NEG_BIG, count > 0 && ok ? l : 0.f);
+        // The results leave through shared memory, a row per copy: stored from the registers they took 10,000 cycles. Both
+        // chains have had their last product when all are here.
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+        if (count > 0 && ok) {
+            uint8_t* mine = ring + (c * ROWS + r) * SH::OUT_ROW;
 #pragma unroll
-            for (int d = 0; d < OHALF; d += 32) {
+            for (int d = 0; d < HD; d += 32) {
                 uint32_t o[32];
                 tmem_ld32(o_addr + d, o);
                 tmem_ld_wait();
-                if (real) {
 #pragma unroll
-                    for (int j = 0; j < 32; j += 4)
-                        *reinterpret_cast<uint4*>(a.part_o + row * HD + half * OHALF + d + j) = make_uint4(o[j], o[j + 1], o[j + 2], o[j + 3]);
-                }
+                for (int j = 0; j < 32; j += 4) *reinterpret_cast<uint4*>(mine + (d + j) * 4) = make_uint4(o[j], o[j + 1], o[j + 2], o[j + 3]);
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            if (real) {
+                asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(a.part_o + row * HD), "r"(smem_u32(mine)), "n"(HD * 4) : "memory");
+                asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+                asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
             }
         }
         tcgen05_fence_before();
@@ -875,7 +849,7 @@ extern "C" int lp_attention_shared(const void* q, void* out, const void* pages, 
     if (B <= 0 || T <= 0 || max_new <= 0 || G <= 0 || H <= 0 || H % G || H / G > ROWS || (hd != 64 && hd != 128) || shared_pages < 0 || shared_pages > width)
         LP_REFUSE("attention_shared: %d sequences, %d tokens, %d heads on %d of %d, %d shared pages", B, T, H, G, hd, shared_pages);
     if (!(scale > 0.f)) LP_REFUSE("attention_shared: a scale of %g", (double)scale);
-    if (splits < 0 || splits > 32 || (splits > 0) != (shared_pages > 0) || splits > (shared_pages + 1) / 2)
+    if (splits < 0 || splits > 32 || (splits > 0) != (shared_pages > 0) || splits > shared_pages)
         LP_REFUSE("attention_shared: %d shares of %d pages", splits, shared_pages);
     if (B > 65535 || G > 65535 || num_pages * 2 * G * PAGE > 0x7fffffffll || ((uintptr_t)q | (uintptr_t)pages | (uintptr_t)out) & 15)
         LP_REFUSE("attention_shared: %d sequences, %lld pages for %d heads, or operands that are not aligned to 16 bytes", B, num_pages, G);

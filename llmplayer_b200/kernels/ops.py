@@ -1321,13 +1321,13 @@ SHARED_SPLITS_MOST = 32
 @functools.lru_cache(maxsize=512)
 def shared_split(tokens: int, num_heads: int, num_kv_heads: int, shared_pages: int):
     """(shares, partial results per row) of the shared pages: a CTA takes two tiles of rows of one key/value head and one share of
-    the blocks of 128 keys. As many shares as make the last round of CTAs end soonest, counting a CTA's start and end as three
-    blocks; a single tile leaves two partial results per share (its CTA's two chains take alternate blocks)."""
+    the pages. As many shares as make the last round of CTAs end soonest, counting a CTA's start and end as six pages; a single
+    tile leaves two partial results per share (its CTA's two chains take alternate pages)."""
     if shared_pages == 0:
         return 0, 0
     tiles = -(-tokens // (SHARED_ROWS // (num_heads // num_kv_heads)))
-    ctas, blocks, sms = -(-tiles // 2) * num_kv_heads, -(-shared_pages // 2), num_sms()
-    best = min(range(1, min(blocks, SHARED_SPLITS_MOST) + 1), key=lambda n: (-(-ctas * n // sms) * (-(-blocks // n) + 3), n))
+    ctas, sms = -(-tiles // 2) * num_kv_heads, num_sms()
+    best = min(range(1, min(shared_pages, SHARED_SPLITS_MOST) + 1), key=lambda n: (-(-ctas * n // sms) * (-(-shared_pages // n) + 6), n))
     return best, (2 * best if tiles == 1 else best)
 
 
