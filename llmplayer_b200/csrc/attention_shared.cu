@@ -19,7 +19,7 @@
 namespace {
 
 constexpr int ROWS = 128;                 // rows of a product: (token, query head) pairs of one key/value head
-constexpr int THREADS = 384;              // warp 0: loader, warp 1: MMA (2 and 3: nothing), warps 4-7 and 8-11: the softmax of the two chains
+constexpr int THREADS = 384;              // warp 0: loader, warps 1 and 2: the chains' products (3: nothing), warps 4-7 and 8-11: their softmaxes
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float RESCALE_ABOVE = 8.0f;     // log2: how far a row's reference maximum may lag behind its maximum (a factor of 256)
 
@@ -165,7 +165,7 @@ attention_shared_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
         asm volatile("prefetch.tensormap [%0];" ::"l"(&map_q) : "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(&map_kv) : "memory");
         mbar_init(q_full, 1);
-        for (int s = 0; s < SLOTS; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
+        for (int s = 0; s < SLOTS; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], alone ? 1 : chains); }
         for (int i = 0; i < 4; ++i) { mbar_init(&s_ready[i], 1); mbar_init(&p_ready[i], 4); }
         mbar_init(&o_ready[0], 1);
         mbar_init(&o_ready[1], 1);
@@ -225,60 +225,55 @@ attention_shared_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
         if (!ok)                                                   // the copies in flight land before the CTA ends
             for (int i = max(0, at - SLOTS); i < at; ++i) mbar_wait(&full[i % SLOTS], (i / SLOTS) & 1);
         __syncwarp();
-    } else if (warp == 1) {
-        // ------------------------------------------------------------ MMA issuer
+    } else if (warp < 3) {
+        // ------------------------------------------------------------ products, a warp per chain
+        // (Waiting and committing cost a warp more than issuing: one warp for both chains took 2,350 cycles per page.)
         constexpr uint32_t base_idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(ROWS >> 4) << 24);
         constexpr uint32_t idesc_s = base_idesc | ((uint32_t)(PAGE >> 3) << 17);
         constexpr uint32_t idesc_pv = base_idesc | (1u << 16) | ((uint32_t)(HD >> 3) << 17);                  // V: contiguous in N
+        const int c = warp - 1, count = turns(c);
         const uint32_t leader = elect_one();
-        const uint64_t desc_q = smem_desc(smem_u32(q_tiles)), desc_k = smem_desc(smem_u32(ring)), desc_v = smem_desc_mn(smem_u32(ring), PAGE * 128);
+        const uint64_t desc_q = smem_desc(smem_u32(q_tiles + (alone ? 0 : c) * SH::Q_TILE)), desc_k = smem_desc(smem_u32(ring));
+        const uint64_t desc_v = smem_desc_mn(smem_u32(ring), PAGE * 128);
+        const uint32_t s_col = tmem_base + SH::S_COL + c * 128, o_col = tmem_base + SH::O_COL + c * HD;
         auto arrived = [&](uint64_t* bar, uint32_t parity, int code) {
             const bool yes = __all_sync(0xffffffffu, mbar_wait(bar, parity));
             if (!yes && leader) atomicExch(a.status, code);
             return yes;
         };
-        bool ok = arrived(q_full, 0, 82);
-        const int turns_of[2] = {turns(0), turns(1)};
-        // the last chain that takes a tile gives its slot back
-        auto last_chain = [&](int c) { return alone || c == chains - 1; };
-        auto scores = [&](int k, int c) -> bool {
+        auto scores = [&](int k) -> bool {
             const int at = keys_at(page_of(k, c)), s = at % SLOTS;
             if (!arrived(&full[s], (at / SLOTS) & 1, 83)) return false;
             tcgen05_fence_after();
-            const uint64_t dq = desc_q + (uint64_t)((alone ? 0 : c) * (SH::Q_TILE >> 4)), dk = desc_k + (uint64_t)(s * (TILE >> 4));
+            const uint64_t dk = desc_k + (uint64_t)(s * (TILE >> 4));
 #pragma unroll
             for (int j = 0; j < HD / 16; ++j)                  // 16 features per instruction; 4 instructions per block of 64
-                mma_ss(leader, tmem_base + SH::S_COL + c * 128 + (k & 1) * PAGE, dq + (uint64_t)((j >> 2) * (ROWS * 128 >> 4) + (j & 3) * 2),
+                mma_ss(leader, s_col + (k & 1) * PAGE, desc_q + (uint64_t)((j >> 2) * (ROWS * 128 >> 4) + (j & 3) * 2),
                        dk + (uint64_t)((j >> 2) * (PAGE * 128 >> 4) + (j & 3) * 2), idesc_s, j > 0 ? 1u : 0u);
             commit(leader, &s_ready[c * 2 + (k & 1)]);
-            if (last_chain(c)) commit(leader, &empty[s]);
+            commit(leader, &empty[s]);
             return true;
         };
-        auto values = [&](int k, int c) -> bool {
+        auto values = [&](int k) -> bool {
             const int at = values_at(page_of(k, c)), s = at % SLOTS;
             if (!arrived(&full[s], (at / SLOTS) & 1, 83) || !arrived(&p_ready[c * 2 + (k & 1)], (k >> 1) & 1, 84)) return false;
             tcgen05_fence_after();
             const uint64_t dv = desc_v + (uint64_t)(s * (TILE >> 4));
-            const uint32_t d = tmem_base + SH::O_COL + c * HD, p = tmem_base + SH::S_COL + c * 128 + (k & 1) * PAGE;
-            mma_ts(leader, d, p, dv, idesc_pv, k > 0 ? 1u : 0u);
 #pragma unroll
-            for (int j = 1; j < PAGE / 16; ++j) mma_ts(leader, d, p + j * 8, dv + (uint64_t)(j * (2048 >> 4)), idesc_pv, 1u);
+            for (int j = 0; j < PAGE / 16; ++j)
+                mma_ts(leader, o_col, s_col + (k & 1) * PAGE + j * 8, dv + (uint64_t)(j * (2048 >> 4)), idesc_pv, (j > 0 || k > 0) ? 1u : 0u);
             commit(leader, &o_ready[c]);
-            if (last_chain(c)) commit(leader, &empty[s]);
+            commit(leader, &empty[s]);
             return true;
         };
         // A chain's scores go over the weights of two pages before, which the products issued before them have read.
-#pragma unroll
+        bool ok = count > 0 && arrived(q_full, 0, 82);
         for (int k = 0; k < 2; ++k)
-#pragma unroll
-            for (int c = 0; c < 2; ++c)
-                if (ok && k < turns_of[c]) ok = scores(k, c);
-        for (int k = 0; k < turns_of[0] && ok; ++k)            // chain 0 has as many turns as chain 1, or one more
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                if (ok && k < turns_of[c]) ok = values(k, c);
-                if (ok && k + 2 < turns_of[c]) ok = scores(k + 2, c);
-            }
+            if (ok && k < count) ok = scores(k);
+        for (int k = 0; k < count && ok; ++k) {
+            ok = values(k);
+            if (ok && k + 2 < count) ok = scores(k + 2);
+        }
         __syncwarp();
     } else if (warp >= 4) {
         // ------------------------------------------------------------ softmax: a thread per row
