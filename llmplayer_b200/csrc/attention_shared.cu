@@ -351,14 +351,17 @@ attention_shared_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
             tmem_st32(s_addr, p);
             tmem_st_wait();
             l += (sum4[0] + sum4[1]) + (sum4[2] + sum4[3]);
+            // A parity tells only a phase from the one before it. The scores of page k say that the products up to page k - 2 have been
+            // added; before the last page's product is let go the one before it is awaited, so that the last can be awaited by itself.
+            if (k > 0 && k == count - 1) {
+                ok = __all_sync(0xffffffffu, mbar_wait(&o_ready[c], (k - 1) & 1));
+                if (!ok) { if (lane == 0) atomicExch(a.status, 86); break; }
+            }
             tcgen05_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&p_ready[c * 2 + (k & 1)]);
         }
-        // The last scores say that all products but two have been added: those two are awaited one by one, as a parity tells only a
-        // phase from the one before it.
-        for (int k = max(0, count - 2); k < count; ++k)
-            if (ok && !__all_sync(0xffffffffu, mbar_wait(&o_ready[c], k & 1))) { if (lane == 0) atomicExch(a.status, 86); ok = false; }
+        if (count > 0 && ok && !__all_sync(0xffffffffu, mbar_wait(&o_ready[c], (count - 1) & 1))) { if (lane == 0) atomicExch(a.status, 86); ok = false; }
         tcgen05_fence_after();
         const int slot = alone ? split * 2 + c : split;
         const long long row = ((long long)slot * a.T + token) * a.H + head;
