@@ -36,45 +36,28 @@ template <int HD> struct Shape {
     static constexpr int BLOCKS = HD / 64;                          // blocks of 64 features (one swizzle row each)
     static constexpr int TILE = PAGE * HD * 2;                      // keys or values of a page
     static constexpr int Q_TILE = ROWS * HD * 2;
-    static constexpr int SLOTS = HD == 64 ? 16 : 10;
+    static constexpr int SLOTS = HD == 64 ? 16 : 8;                 // a power of two: which slot and which round are bits of a tile's place
     static constexpr int SMEM = 2 * Q_TILE + SLOTS * TILE + 1024 /* alignment */ + 512 /* barriers */ + 2 * ROWS * 4 /* positions */;
-    static constexpr int OUT_ROW = HD * 4 + 16;                     // a row of results on its way out: where the ring was
-    static_assert(SMEM <= 227 * 1024 && 2 * ROWS * OUT_ROW <= SLOTS * TILE, "");
+    static constexpr int OUT_ROW = HD * 4 + 16;                     // a row of results on its way out: where queries and ring were
+    static_assert(SMEM <= 227 * 1024 && 2 * ROWS * OUT_ROW <= 2 * Q_TILE + SLOTS * TILE && (SLOTS & (SLOTS - 1)) == 0, "");
     static constexpr int S_COL = 0, O_COL = 256;                    // chain c: S at 128 c and 128 c + 64, O at 256 + HD c
     static constexpr int TMEM_COLS = 512;
 };
 
-// The products' issue by a whole warp of which one thread is elected: with values that the compiler knows to be alike in all lanes the
-// descriptors stay in uniform registers. Issued from a branch of one lane, an instruction took about 100 cycles, and the issue of a
-// block's products (5,000 cycles) was all that the kernel waited for.
-__device__ __forceinline__ uint32_t elect_one() {
+// The products are issued by a whole warp of which one thread is elected: values that the compiler knows to be alike in all lanes stay
+// in uniform registers.
+__device__ __forceinline__ bool elect_one() {
     uint32_t leader;
     asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(leader));
-    return leader;
+    return leader != 0;
 }
-__device__ __forceinline__ void mma_ss(uint32_t leader, uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
+// A product whose first operand lies in tensor memory.
+__device__ __forceinline__ void mma_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
-        "{\n\t.reg .pred p, q;\n\t"
+        "{\n\t.reg .pred p;\n\t"
         "setp.ne.b32 p, %4, 0;\n\t"
-        "setp.ne.b32 q, %5, 0;\n\t"
-        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-        ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate), "r"(leader) : "memory");
-}
-// the first operand in tensor memory
-__device__ __forceinline__ void mma_ts(uint32_t leader, uint32_t tmem_d, uint32_t tmem_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p, q;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "setp.ne.b32 q, %5, 0;\n\t"
-        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
-        ::"r"(tmem_d), "r"(tmem_a), "l"(desc_b), "r"(idesc), "r"(accumulate), "r"(leader) : "memory");
-}
-__device__ __forceinline__ void commit(uint32_t leader, uint64_t* bar) {
-    asm volatile(
-        "{\n\t.reg .pred q;\n\t"
-        "setp.ne.b32 q, %1, 0;\n\t"
-        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}"
-        ::"r"(smem_u32(bar)), "r"(leader) : "memory");
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+        ::"r"(tmem_d), "r"(tmem_a), "l"(desc_b), "r"(idesc), "r"(accumulate) : "memory");
 }
 __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
     asm volatile(
@@ -232,47 +215,51 @@ attention_shared_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
         constexpr uint32_t idesc_s = base_idesc | ((uint32_t)(PAGE >> 3) << 17);
         constexpr uint32_t idesc_pv = base_idesc | (1u << 16) | ((uint32_t)(HD >> 3) << 17);                  // V: contiguous in N
         const int c = warp - 1, count = turns(c);
-        const uint32_t leader = elect_one();
+        const bool leader = elect_one();
         const uint64_t desc_q = smem_desc(smem_u32(q_tiles + (alone ? 0 : c) * SH::Q_TILE)), desc_k = smem_desc(smem_u32(ring));
         const uint64_t desc_v = smem_desc_mn(smem_u32(ring), PAGE * 128);
         const uint32_t s_col = tmem_base + SH::S_COL + c * 128, o_col = tmem_base + SH::O_COL + c * HD;
-        auto arrived = [&](uint64_t* bar, uint32_t parity, int code) {
-            const bool yes = __all_sync(0xffffffffu, mbar_wait(bar, parity));
-            if (!yes && leader) atomicExch(a.status, code);
-            return yes;
+        bool ok = count > 0;
+        auto await = [&](uint64_t* bar, uint32_t parity, int code) {
+            if (!mbar_test(bar, parity) && !mbar_wait(bar, parity)) { ok = false; atomicExch(a.status, code); }
         };
-        auto scores = [&](int k) -> bool {
+        auto scores = [&](int k) {
             const int at = keys_at(page_of(k, c)), s = at % SLOTS;
-            if (!arrived(&full[s], (at / SLOTS) & 1, 83)) return false;
+            await(&full[s], (at / SLOTS) & 1, 83);
             tcgen05_fence_after();
             const uint64_t dk = desc_k + (uint64_t)(s * (TILE >> 4));
+            if (ok && leader) {
 #pragma unroll
-            for (int j = 0; j < HD / 16; ++j)                  // 16 features per instruction; 4 instructions per block of 64
-                mma_ss(leader, s_col + (k & 1) * PAGE, desc_q + (uint64_t)((j >> 2) * (ROWS * 128 >> 4) + (j & 3) * 2),
-                       dk + (uint64_t)((j >> 2) * (PAGE * 128 >> 4) + (j & 3) * 2), idesc_s, j > 0 ? 1u : 0u);
-            commit(leader, &s_ready[c * 2 + (k & 1)]);
-            commit(leader, &empty[s]);
-            return true;
+                for (int j = 0; j < HD / 16; ++j)              // 16 features per instruction; 4 instructions per block of 64
+                    tcgen05_mma(s_col + (k & 1) * PAGE, desc_q + (uint64_t)((j >> 2) * (ROWS * 128 >> 4) + (j & 3) * 2),
+                                dk + (uint64_t)((j >> 2) * (PAGE * 128 >> 4) + (j & 3) * 2), idesc_s, j > 0 ? 1u : 0u);
+                tcgen05_commit(&s_ready[c * 2 + (k & 1)]);
+                tcgen05_commit(&empty[s]);
+            }
+            __syncwarp();
         };
-        auto values = [&](int k) -> bool {
+        auto values = [&](int k) {
             const int at = values_at(page_of(k, c)), s = at % SLOTS;
-            if (!arrived(&full[s], (at / SLOTS) & 1, 83) || !arrived(&p_ready[c * 2 + (k & 1)], (k >> 1) & 1, 84)) return false;
-            tcgen05_fence_after();
+            await(&full[s], (at / SLOTS) & 1, 83);
             const uint64_t dv = desc_v + (uint64_t)(s * (TILE >> 4));
+            await(&p_ready[c * 2 + (k & 1)], (k >> 1) & 1, 84);
+            tcgen05_fence_after();
+            if (ok && leader) {
 #pragma unroll
-            for (int j = 0; j < PAGE / 16; ++j)
-                mma_ts(leader, o_col, s_col + (k & 1) * PAGE + j * 8, dv + (uint64_t)(j * (2048 >> 4)), idesc_pv, (j > 0 || k > 0) ? 1u : 0u);
-            commit(leader, &o_ready[c]);
-            commit(leader, &empty[s]);
-            return true;
+                for (int j = 0; j < PAGE / 16; ++j)
+                    mma_ts(o_col, s_col + (k & 1) * PAGE + j * 8, dv + (uint64_t)(j * (2048 >> 4)), idesc_pv, (j > 0 || k > 0) ? 1u : 0u);
+                tcgen05_commit(&o_ready[c]);
+                tcgen05_commit(&empty[s]);
+            }
+            __syncwarp();
         };
         // A chain's scores go over the weights of two pages before, which the products issued before them have read.
-        bool ok = count > 0 && arrived(q_full, 0, 82);
+        if (ok) await(q_full, 0, 82);
         for (int k = 0; k < 2; ++k)
-            if (ok && k < count) ok = scores(k);
-        for (int k = 0; k < count && ok; ++k) {
-            ok = values(k);
-            if (ok && k + 2 < count) ok = scores(k + 2);
+            if (__all_sync(0xffffffffu, ok) && k < count) scores(k);
+        for (int k = 0; k < count && __all_sync(0xffffffffu, ok); ++k) {
+            values(k);
+            if (k + 2 < count) scores(k + 2);
         }
         __syncwarp();
     } else if (warp >= 4) {
@@ -370,7 +357,7 @@ attention_shared_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
         // chains have had their last product when all are here.
         asm volatile("bar.sync 1, 256;" ::: "memory");
         if (count > 0 && ok) {
-            uint8_t* mine = ring + (c * ROWS + r) * SH::OUT_ROW;
+            uint8_t* mine = q_tiles + (c * ROWS + r) * SH::OUT_ROW;
 #pragma unroll
             for (int d = 0; d < HD; d += 32) {
                 uint32_t o[32];
