@@ -419,36 +419,53 @@ __device__ __forceinline__ void clear_values(uint8_t* v_tile, int from, int to, 
 }
 
 // A single new token per sequence: the keys are the rows of the products and the (up to 8) query heads of a key/value head their
-// columns (see attention_decode.cuh); four warps share a page, 16 keys each. grid: (G x head groups, B); 128 threads.
+// columns (see attention_decode.cuh); four warps share a page, 16 keys each. grid: (G x head groups, B); 128 threads. Keys and values of a
+// page come one by one through a ring of three tiles (two pages at heads of 64), so that four CTAs share an SM at heads of 128.
 template <int HD> struct OwnShape {
-    static constexpr int STAGE = 2 * PAGE * HD * 2;
-    static constexpr int STAGES = HD == 64 ? 4 : 2;
-    static constexpr int SMEM = STAGES * STAGE + 1024;
-    static_assert(STAGES * STAGE >= (4 * HEAD_ROWS * (HD + 2)) * 4, "the warps' results lie where the pages were");
+    static constexpr int TILE = PAGE * HD * 2;
+    static constexpr int TILES = HD == 64 ? 4 : 3;
+    static constexpr int SMEM = TILES * TILE + 1024;
+    static_assert(TILES * TILE >= 4 * HEAD_ROWS * (HD + 2) * 4, "the warps' results lie where the pages were");
 };
+constexpr int MOST_SLOTS = 64;
 template <int HD>
 __global__ void __launch_bounds__(128)
 attention_own_single_kernel(const __grid_constant__ CUtensorMap map_kv, const OwnArgs a) {
     using SH = OwnShape<HD>;
-    constexpr int KSTEPS = HD / 16, STAGES = SH::STAGES, MOST_SLOTS = 64;
+    constexpr int KSTEPS = HD / 16, TILES = SH::TILES, TILE = SH::TILE;
     extern __shared__ __align__(128) uint8_t smem_raw[];
     uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-    __shared__ __align__(8) uint64_t full[STAGES];
+    __shared__ __align__(8) uint64_t full[TILES];
     __shared__ float factor[HEAD_ROWS][MOST_SLOTS + 4];
     __shared__ float total[HEAD_ROWS];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int b = blockIdx.y, groups = gridDim.x / a.G, g = blockIdx.x / groups, hg = blockIdx.x - g * groups;
     const int head0 = g * a.R + hg * HEAD_ROWS, nrows = min(HEAD_ROWS, a.R - hg * HEAD_ROWS);
     if (a.waits_first) lp_grid_wait();
-    const int t = a.q_start[b];
-    const bool real = a.q_start[b + 1] > t && t >= 0 && t < a.T;   // one new token, or none
-    const int pos = real ? a.kv_len[b] - 1 : -1;
-    const int last = pos >= 0 ? pos / PAGE : -1, npages = max(0, min(last + 1, a.width) - a.pages);
     const int* table = a.table + (long long)b * a.width + a.pages;
-    if (tid == 0) {
-        for (int s = 0; s < STAGES; ++s) mbar_init(&full[s], 1);
-        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-        for (int p = 0; p < STAGES && p < npages; ++p) request_page<HD>(smem + p * SH::STAGE, &full[p], &map_kv, table[p], a.G, g);
+    // asked for together; the first own pages' numbers as well (a sequence without any has none there to use)
+    const int t = a.q_start[b], t_end = a.q_start[b + 1], len = a.kv_len[b];
+    const int held = lane < a.width - a.pages ? table[lane] : 0;
+    const bool real = t_end > t && t >= 0 && t < a.T;              // one new token, or none
+    const int pos = real ? len - 1 : -1;
+    const int last = pos >= 0 ? pos / PAGE : -1, npages = max(0, min(last + 1, a.width) - a.pages);
+    auto request = [&](int n) {                                    // by the whole first warp: tile n = keys or values of page n / 2
+        const int p = n >> 1, page = p < 32 ? __shfl_sync(0xffffffffu, held, p) : table[p];
+        if (lane == 0) {
+            uint64_t* bar = &full[n % TILES];
+            mbar_expect_tx(bar, TILE);
+#pragma unroll
+            for (int f = 0; f < HD / 64; ++f)
+                tma_load_2d(smem + (n % TILES) * TILE + f * (PAGE * 128), &map_kv, f * 64, ((page * 2 + (n & 1)) * a.G + g) * PAGE, bar);
+        }
+    };
+    if (warp == 0) {
+        if (lane == 0) {
+            for (int s = 0; s < TILES; ++s) mbar_init(&full[s], 1);
+            asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        }
+        __syncwarp();
+        for (int n = 0; n < TILES && n < 2 * npages; ++n) request(n);
     }
     __syncthreads();
     const int g8 = lane >> 2, t4 = lane & 3;
@@ -466,23 +483,41 @@ attention_own_single_kernel(const __grid_constant__ CUtensorMap map_kv, const Ow
     for (int i = 0; i < KSTEPS; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
     float m0 = NEG_BIG, m1 = NEG_BIG, l0 = 0.f, l1 = 0.f;          // of heads 2 t4 and 2 t4 + 1
     const int frag_row = (lane & 7) + ((lane >> 3) & 1) * 8, frag_chunk = lane >> 4, key0 = warp * 16;
+    auto arrived = [&](int n) {
+        const bool yes = mbar_wait(&full[n % TILES], (n / TILES) & 1);
+        if (!yes && lane == 0) atomicExch(a.status, 87);
+        return yes;
+    };
+    auto refill = [&](int n) {                                     // tile n has been read by all: tile n + TILES goes there
+        __syncthreads();
+        if (warp == 0 && n + TILES < 2 * npages) {
+            // what was written here by stores comes before what the copy writes
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            request(n + TILES);
+        }
+    };
     for (int p = 0; p < npages; ++p) {
-        uint8_t* stage = smem + (p % STAGES) * SH::STAGE;
-        const bool arrived = mbar_wait(&full[p % STAGES], (p / STAGES) & 1);
-        if (!arrived && lane == 0) atomicExch(a.status, 87);
         const int key_base = (a.pages + p) * PAGE;
-        if (arrived && key_base + key0 <= pos) {
-            const uint32_t k_tile = smem_u32(stage), v_tile = k_tile + PAGE * HD * 2;
-            if (key_base + key0 + 15 > pos) {                      // the warp's own rows of the page
-                clear_values<HD>(stage + PAGE * HD * 2, pos + 1 - key_base, key0 + 16, lane, 32);
-                __syncwarp();
-            }
-            float s[4] = {0.f, 0.f, 0.f, 0.f};
+        const bool active = key_base + key0 <= pos;
+        float s[4] = {0.f, 0.f, 0.f, 0.f};
+        bool there = arrived(2 * p);
+        if (there && active) {
+            const uint32_t k_tile = smem_u32(smem + (2 * p % TILES) * TILE);
 #pragma unroll
             for (int kk = 0; kk < KSTEPS; ++kk) {
                 uint32_t x[4];
                 ldmatrix_x4(k_tile + tile_offset<true>(key0 + frag_row, kk * 2 + frag_chunk, HD, HD / 8), x[0], x[1], x[2], x[3]);
                 mma_bf16(s, x, qf[kk][0], qf[kk][1]);
+            }
+        }
+        refill(2 * p);
+        there = arrived(2 * p + 1) && there;
+        if (there && active) {
+            uint8_t* values = smem + ((2 * p + 1) % TILES) * TILE;
+            const uint32_t v_tile = smem_u32(values);
+            if (key_base + key0 + 15 > pos) {                      // the warp's own rows of the page
+                clear_values<HD>(values, pos + 1 - key_base, key0 + 16, lane, 32);
+                __syncwarp();
             }
             const bool out_a = key_base + key0 + g8 > pos, out_b = key_base + key0 + g8 + 8 > pos;
             s[0] = out_a ? NEG_BIG : s[0] * a.scale_log2;
@@ -512,12 +547,7 @@ attention_own_single_kernel(const __grid_constant__ CUtensorMap map_kv, const Ow
                 mma_bf16(o[mt], x, p0, p1);
             }
         }
-        __syncthreads();
-        if (tid == 0 && p + STAGES < npages) {
-            // what was written here by stores comes before what the copy writes
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            request_page<HD>(stage, &full[p % STAGES], &map_kv, table[p + STAGES], a.G, g);
-        }
+        refill(2 * p + 1);
     }
 #pragma unroll
     for (int sh = 4; sh < 32; sh <<= 1) {
@@ -544,48 +574,54 @@ attention_own_single_kernel(const __grid_constant__ CUtensorMap map_kv, const Ow
     if (!real) return;
     // per head the factor of each partial result: the four warps' and the shared pages'
     for (int r = warp; r < nrows; r += 4) {
-        const float* ml = a.part_ml + ((long long)t * a.H + head0 + r) * 2;
-        const long long step = (long long)a.T * a.H * 2;
-        float m = NEG_BIG, l = 0.f, mine[(MOST_SLOTS + 4 + 31) / 32];
+        const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + (long long)t * a.H + head0 + r;
+        const long long step = (long long)a.T * a.H;
+        constexpr int PER = (MOST_SLOTS + 4 + 31) / 32;
+        float mi[PER], li[PER], m = NEG_BIG, l = 0.f;
 #pragma unroll
-        for (int k = 0; k < (MOST_SLOTS + 4 + 31) / 32; ++k) {
+        for (int k = 0; k < PER; ++k) {
             const int i = k * 32 + lane;
-            float mi = NEG_BIG, li = 0.f;
-            if (i < 4) { mi = sm_m[i * HEAD_ROWS + r]; li = sm_l[i * HEAD_ROWS + r]; }
-            else if (i < 4 + a.slots) { mi = __ldcg(ml + (i - 4) * step); li = __ldcg(ml + (i - 4) * step + 1); }
-            if (!(li > 0.f) && li == li) mi = NEG_BIG;             // nothing there (no number passes through)
-            const float most = lp_warp_max(mi), before = m;
-            m = fmaxf(m, most);
-            l = l * fast_exp2(before - m);
-#pragma unroll
-            for (int j = 0; j < k; ++j) mine[j] *= fast_exp2(before - m);
-            mine[k] = li != 0.f ? fast_exp2(mi - m) : 0.f;
-            l += lp_warp_sum(li * mine[k]);
+            float2 x = make_float2(NEG_BIG, 0.f);
+            if (i < 4) x = make_float2(sm_m[i * HEAD_ROWS + r], sm_l[i * HEAD_ROWS + r]);
+            else if (i < 4 + a.slots) x = __ldcg(ml + (i - 4) * step);
+            mi[k] = x.x;
+            li[k] = x.y;
         }
 #pragma unroll
-        for (int k = 0; k < (MOST_SLOTS + 4 + 31) / 32; ++k)
-            if (k * 32 + lane < 4 + a.slots) factor[r][k * 32 + lane] = mine[k];
+        for (int k = 0; k < PER; ++k) m = fmaxf(m, li[k] != 0.f ? mi[k] : NEG_BIG);      // nothing lies where the sum is zero
+        m = lp_warp_max(m);
+#pragma unroll
+        for (int k = 0; k < PER; ++k) {
+            const float f = li[k] != 0.f ? fast_exp2(mi[k] - m) : 0.f;
+            l += li[k] * f;
+            if (k * 32 + lane < 4 + a.slots) factor[r][k * 32 + lane] = f;
+        }
+        l = lp_warp_sum(l);
         if (lane == 0) total[r] = l;
     }
     __syncthreads();
-    for (int idx = tid; idx < nrows * HD; idx += 128) {
-        const int r = idx / HD, d = idx - r * HD;
+    for (int idx = tid; idx < nrows * (HD / 4); idx += 128) {      // four features per thread; sixteen results are asked for at a time
+        const int r = idx / (HD / 4), d = (idx - r * (HD / 4)) * 4;
         const float* po = a.part_o + ((long long)t * a.H + head0 + r) * HD + d;
         const long long step = (long long)a.T * a.H * HD;
-        float acc = 0.f;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        auto add = [&](const float4& x, float f) {
+            acc.x += x.x * f; acc.y += x.y * f; acc.z += x.z * f; acc.w += x.w * f;
+        };
 #pragma unroll
-        for (int w = 0; w < 4; ++w)
-            if (factor[r][w] != 0.f) acc += sm_o[(w * HEAD_ROWS + r) * HD + d] * factor[r][w];
-        for (int s0 = 0; s0 < a.slots; s0 += 8) {
-            float x[8];
+        for (int w = 0; w < 4; ++w) add(*reinterpret_cast<const float4*>(&sm_o[(w * HEAD_ROWS + r) * HD + d]), factor[r][w]);
+        for (int s0 = 0; s0 < a.slots; s0 += 16) {
+            float4 x[16];
 #pragma unroll
-            for (int u = 0; u < 8; ++u) x[u] = s0 + u < a.slots && factor[r][4 + s0 + u] != 0.f ? __ldcg(po + (s0 + u) * step) : 0.f;
+            for (int u = 0; u < 16; ++u)
+                x[u] = s0 + u < a.slots && factor[r][4 + s0 + u] != 0.f ? __ldcg(reinterpret_cast<const float4*>(po + (s0 + u) * step)) : make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-            for (int u = 0; u < 8; ++u)
-                if (s0 + u < a.slots) acc += x[u] * factor[r][4 + s0 + u];
+            for (int u = 0; u < 16; ++u)
+                if (s0 + u < a.slots) add(x[u], factor[r][4 + s0 + u]);
         }
-        const float l = total[r];
-        a.out[((long long)t * a.H + head0 + r) * HD + d] = __float2bfloat16_rn(l > 0.f || l != l ? acc / l : 0.f);
+        const float l = total[r], inv = l != 0.f ? 1.0f / l : 0.f;
+        uint2 packed = l != 0.f ? make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv)) : make_uint2(0, 0);
+        *reinterpret_cast<uint2*>(a.out + ((long long)t * a.H + head0 + r) * HD + d) = packed;
     }
 }
 
