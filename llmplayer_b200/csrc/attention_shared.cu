@@ -136,13 +136,16 @@ attention_shared_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
     const int chains = alone || pair * 2 + 1 < tiles ? 2 : 1;
     const int t0 = pair * 2 * per_tile;
     const int first = (int)((long long)a.pages * split / a.splits), n = (int)((long long)a.pages * (split + 1) / a.splits) - first;
-    // A chain's k-th page is page k of the share, or every second one. Tiles are asked for in the order in which the products take
-    // them: `lead` pages' keys, then the values of a page and the keys of the page `lead` behind it.
-    const int step = alone ? 2 : 1, lead = 2 * step;
+    // A chain's k-th page is page k of the share, or every second one. Tiles come in the order in which the products take them: two
+    // pages' keys, then the values of a page and the keys of the page two behind it. Chains that take alternate pages have half of the
+    // slots each: whoever waits for a slot's tile must have seen the tile before it there, as a parity tells only a round from the last.
+    const int streams = alone ? 2 : 1, slots = SLOTS / streams, slots_log2 = 31 - __clz(slots);
     auto page_of = [&](int k, int c) { return alone ? 2 * k + c : k; };
     auto turns = [&](int c) { return alone ? (n + 1 - c) / 2 : c < chains ? n : 0; };
-    auto keys_at = [&](int i) { return i < lead ? i : 2 * i - lead + 1; };
-    auto values_at = [&](int i) { return min(n, lead + i) + i; };
+    auto keys_at = [&](int k) { return k < 2 ? k : 2 * k - 1; };
+    auto values_at = [&](int k, int count) { return min(count, 2 + k) + k; };
+    auto slot_of = [&](int at, int c) { return (alone ? c * slots : 0) + (at & (slots - 1)); };
+    auto round_of = [&](int at) { return (at >> slots_log2) & 1; };
 
     if (threadIdx.x == 0) {
         asm volatile("prefetch.tensormap [%0];" ::"l"(&map_q) : "memory");
@@ -178,19 +181,19 @@ attention_shared_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
         }
         // The lanes hold page numbers (lane j those of pages j, j + 32, ... of the share, the last two of them), so that a request does not
         // begin with a round trip to memory.
-        int held = lane < n ? a.table[first + lane] : 0, before = 0;
-        int loaded = 32;
+        int held = lane < n ? a.table[first + lane] : 0, before = 0, loaded = 32;
+        int at[2] = {0, 0};                                        // tiles asked for, per stream
         bool ok = true;
-        int at = 0;
-        auto request = [&](int i, int which) {
+        auto request = [&](int k, int c, int which) {
+            const int i = page_of(k, c);
             if (i >= loaded) {                                     // keys run ahead of values by less than 32 pages
                 before = held;
                 held = loaded + lane < n ? a.table[first + loaded + lane] : 0;
                 loaded += 32;
             }
             const int page = __shfl_sync(0xffffffffu, i >= loaded - 32 ? held : before, i & 31);
-            const int s = at % SLOTS;
-            ok = __all_sync(0xffffffffu, mbar_wait(&empty[s], ((at / SLOTS) & 1) ^ 1));
+            const int s = slot_of(at[c], c);
+            ok = __all_sync(0xffffffffu, mbar_wait(&empty[s], round_of(at[c]) ^ 1));
             if (!ok) { if (lane == 0) atomicExch(a.status, 81); return; }
             if (lane == 0) {
                 mbar_expect_tx(&full[s], (uint32_t)TILE);
@@ -198,15 +201,23 @@ attention_shared_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
 #pragma unroll
                 for (int f = 0; f < SH::BLOCKS; ++f) tma_load_2d(ring + s * TILE + f * (PAGE * 128), &map_kv, f * 64, row, &full[s]);
             }
-            ++at;
+            ++at[c];
         };
-        for (int i = 0; i < min(lead, n) && ok; ++i) request(i, 0);
-        for (int i = 0; i < n && ok; ++i) {
-            request(i, 1);
-            if (ok && i + lead < n) request(i + lead, 0);
-        }
+        const int counts[2] = {turns(0), streams == 2 ? turns(1) : 0};
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+            for (int c = 0; c < 2; ++c)
+                if (ok && k < counts[c]) request(k, c, 0);
+        for (int k = 0; k < counts[0] && ok; ++k)                  // the first stream has as many pages as the second, or one more
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                if (ok && k < counts[c]) request(k, c, 1);
+                if (ok && k + 2 < counts[c]) request(k + 2, c, 0);
+            }
         if (!ok)                                                   // the copies in flight land before the CTA ends
-            for (int i = max(0, at - SLOTS); i < at; ++i) mbar_wait(&full[i % SLOTS], (i / SLOTS) & 1);
+#pragma unroll
+            for (int c = 0; c < 2; ++c)
+                for (int i = max(0, at[c] - slots); i < at[c]; ++i) mbar_wait(&full[slot_of(i, c)], round_of(i));
         __syncwarp();
     } else if (warp < 3) {
         // ------------------------------------------------------------ products, a warp per chain
@@ -224,8 +235,8 @@ attention_shared_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
             if (!mbar_test(bar, parity) && !mbar_wait(bar, parity)) { ok = false; atomicExch(a.status, code); }
         };
         auto scores = [&](int k) {
-            const int at = keys_at(page_of(k, c)), s = at % SLOTS;
-            await(&full[s], (at / SLOTS) & 1, 83);
+            const int at = keys_at(k), s = slot_of(at, c);
+            await(&full[s], round_of(at), 83);
             tcgen05_fence_after();
             const uint64_t dk = desc_k + (uint64_t)(s * (TILE >> 4));
             if (ok && leader) {
@@ -239,8 +250,8 @@ attention_shared_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
             __syncwarp();
         };
         auto values = [&](int k) {
-            const int at = values_at(page_of(k, c)), s = at % SLOTS;
-            await(&full[s], (at / SLOTS) & 1, 83);
+            const int at = values_at(k, count), s = slot_of(at, c);
+            await(&full[s], round_of(at), 83);
             const uint64_t dv = desc_v + (uint64_t)(s * (TILE >> 4));
             await(&p_ready[c * 2 + (k & 1)], (k >> 1) & 1, 84);
             tcgen05_fence_after();

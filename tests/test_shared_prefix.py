@@ -286,6 +286,16 @@ def test_the_same_pages_many_times_over_and_long_ones():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("tokens", [1, 9, 32])
+@pytest.mark.parametrize("shared", [40, 401, 1100])
+def test_one_tile_of_rows_over_many_pages(shared, tokens, hd):
+    """The rows fill one tile (or less): a CTA's two halves take alternate pages, tens of them each."""
+    check(batch(shared, [shared * PAGE + 1 + i for i in range(tokens)], [1] * tokens, 32, 8, hd, seed=tokens), shared, 32, 8, hd, "shared prefix, single tokens",
+          f"{tokens} tokens on {shared} pages")
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("new", [1, 12])
 def test_results_repeat_and_graphs_replay(new):
     shared, B, H, G, hd = 20, 9, 32, 8, 64
