@@ -1321,14 +1321,17 @@ SHARED_SPLITS_MOST = 32
 @functools.lru_cache(maxsize=512)
 def shared_split(tokens: int, num_heads: int, num_kv_heads: int, shared_pages: int):
     """(shares, partial results per row) of the shared pages: a CTA takes two tiles of rows of one key/value head and one share of
-    the pages. As many shares as make the last round of CTAs end soonest, counting a CTA's start and end as six pages; a single
-    tile leaves two partial results per share (its CTA's two chains take alternate pages)."""
+    the pages. With a single tile its two chains take alternate pages and leave a result each. The shares are those with the
+    least time in pages of a chain: the last round of CTAs ends after its pages and six for a CTA's start and end, and every result is
+    written and read again at 0.4 of a page. (B200, 32 heads of 128 on 8: 16 sequences on 128 pages 24.5 us with 8 to 10 shares, 28.7 with
+    16; 64 sequences 36.9 with 10 to 18, 41 with 8; 200 sequences on 200 pages 92 with 4, 106 with 3.)"""
     if shared_pages == 0:
         return 0, 0
     tiles = -(-tokens // (SHARED_ROWS // (num_heads // num_kv_heads)))
-    ctas, sms = -(-tiles // 2) * num_kv_heads, num_sms()
-    best = min(range(1, min(shared_pages, SHARED_SPLITS_MOST) + 1), key=lambda n: (-(-ctas * n // sms) * (-(-shared_pages // n) + 6), n))
-    return best, (2 * best if tiles == 1 else best)
+    ctas, sms, chains = -(-tiles // 2) * num_kv_heads, num_sms(), 2 if tiles == 1 else 1
+    best = min(range(1, min(shared_pages, SHARED_SPLITS_MOST) + 1),
+               key=lambda n: (-(-ctas * n // sms) * (-(-shared_pages // (n * chains)) + 6) + 0.4 * n * chains, n))
+    return best, best * chains
 
 
 # --------------------------------------------------------------------------- a step's tables, copies of pages
