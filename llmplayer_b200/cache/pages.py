@@ -11,7 +11,7 @@ did not write.
 """
 from __future__ import annotations
 
-from typing import Dict, List, Optional
+from typing import Dict, List, Optional, Tuple
 
 from ..errors import CacheError, CacheFull
 
@@ -64,6 +64,8 @@ class PageMap:
     can reach; ``None`` keeps every page until the slot is released. ``keep_first``: the pages
     that hold a sequence's first so many positions are never given back before that. ``chunk``: no
     later query reaches positions before the start of its own chunk of so many positions.
+
+    A slot that was forked shares the pages that were full then; each goes back when the last of its slots lets go of it.
     """
 
     def __init__(self, num_pages: int, window: Optional[int] = None, page_size: int = PAGE_SIZE, keep_first: int = 0,
@@ -74,6 +76,7 @@ class PageMap:
         self.keep_first = max(0, int(keep_first or 0))
         self.pool = FreeList(num_pages, "page")
         self._pages: Dict[int, List[int]] = {}     # slot -> page id per block of positions (-1: given back)
+        self._others: Dict[int, int] = {}          # page -> how many slots hold it besides one
 
     def open(self, slot: int) -> None:
         if slot in self._pages:
@@ -96,6 +99,33 @@ class PageMap:
         for _ in range(need):
             pages.append(self.pool.take())
 
+    def _let_go(self, page: int) -> None:
+        others = self._others.get(page, 0)
+        if others == 0:
+            self.pool.give_back(page)
+        elif others == 1:
+            del self._others[page]
+        else:
+            self._others[page] = others - 1
+
+    def fork_needs(self, length: int) -> int:
+        """Pages of its own that a fork at ``length`` takes: a copy of the page that is still being filled."""
+        return 1 if length % self.page_size else 0
+
+    def fork(self, slot: int, new: int, length: int) -> Optional[Tuple[int, int]]:
+        """Slot ``new`` holds what ``slot`` holds of positions [0, length): the full pages are shared. Returns (page, copy) if the last
+        page is not full: the caller copies its content."""
+        if new in self._pages:
+            raise CacheError(f"slot {new} already has pages in this group")
+        pages = self._pages[slot]
+        full = length // self.page_size
+        copy = self.pool.take() if self.fork_needs(length) else None
+        for page in pages[:full]:
+            if page >= 0:
+                self._others[page] = self._others.get(page, 0) + 1
+        self._pages[new] = pages[:full] + ([copy] if copy is not None else [])
+        return None if copy is None else (pages[full], copy)
+
     def trim(self, slot: int, length: int) -> None:
         """After a step that left ``slot`` at ``length``: give back the pages whose
         positions all lie before the window (or the chunk) of the next query (position ``length``)."""
@@ -108,13 +138,13 @@ class PageMap:
         kept = -(-self.keep_first // self.page_size)          # blocks that hold the positions kept for good
         for block in range(kept, min(len(pages), max(0, first_needed) // self.page_size)):
             if pages[block] >= 0:
-                self.pool.give_back(pages[block])
+                self._let_go(pages[block])
                 pages[block] = -1
 
     def close(self, slot: int) -> None:
         for page in self._pages.pop(slot):
             if page >= 0:
-                self.pool.give_back(page)
+                self._let_go(page)
 
     def table(self, slot: int) -> List[int]:
         return self._pages[slot]

@@ -23,6 +23,7 @@ from typing import Dict, List, Optional, Sequence, Tuple
 import torch
 
 from ..errors import CacheError, CacheFull
+from ..kernels import ops
 from .pages import PAGE_SIZE, FreeList, PageMap
 
 
@@ -186,6 +187,58 @@ class SequenceCache:
         for rows in self._state_rows:
             rows[slot].zero_()
         return slot
+
+    def fork(self, slot: int, count: int) -> List[int]:
+        """``count`` new slots that hold what ``slot`` holds: full pages are shared (no slot writes to them again), the page that is
+        still being filled and the state rows are copied. All or nothing."""
+        length = self.length(slot)
+        if count < 0:
+            raise CacheError(f"cannot fork slot {slot} {count} times")
+        if count > self.slots.num_free:
+            raise CacheFull(f"{count} forks of slot {slot}: {self.slots.num_free} of {self.max_slots} slots are free")
+        for group in self.groups:
+            need = count * group.pages.fork_needs(length)
+            if need > group.pages.pool.num_free:
+                raise CacheFull(f"the cache is full: {count} forks of slot {slot} need {need} page(s) of {PAGE_SIZE} positions, "
+                                f"{group.pages.pool.num_free} of {group.pages.pool.count} are free")
+        new = [self.slots.take() for _ in range(count)]
+        for s in new:
+            self._length[s] = length
+        for group in self.groups:
+            copies = [pair for pair in (group.pages.fork(slot, s, length) for s in new) if pair is not None]
+            if not copies:
+                continue
+            sources, targets = [a for a, _ in copies], [b for _, b in copies]
+            if group.storage.is_cuda:
+                ops.copy_pages(group.storage, sources, targets)
+            else:
+                group.storage[:, targets] = group.storage[:, sources]
+        if new and self._state_rows:
+            places = torch.tensor(new, device=self.device)
+            for rows in self._state_rows:
+                rows[places] = rows[slot].clone()
+        return new
+
+    def shared_pages(self, slots: Sequence[int]) -> List[int]:
+        """Per group: how many first pages the slots have in common (0 where pages are given back behind a window or a chunk, and for
+        a single slot)."""
+        out = []
+        for group in self.groups:
+            if len(slots) < 2 or group.pages.window is not None or group.pages.chunk is not None:
+                out.append(0)
+                continue
+            first = group.pages.table(slots[0])
+            common = min(len(first), min(self._length[s] for s in slots) // PAGE_SIZE)
+            for s in slots[1:]:
+                table = group.pages.table(s)
+                if not common or not table or table[0] != first[0]:
+                    common = 0
+                    break
+                common = min(common, len(table))
+                if table[:common] != first[:common]:
+                    common = next(i for i in range(common) if table[i] != first[i])
+            out.append(common)
+        return out
 
     def release(self, slot: int) -> None:
         if not self.slots.is_held(slot):

@@ -36,6 +36,8 @@ Options:
   --stop-ids <ids>         Token ids that end a sequence (default: the model's eos_token_id)
   --dtype <name>           bfloat16 (default) or float32
   --max-slots <num>        Sequences held at once (default: one per prompt)
+  --samples <num>          Samples of each prompt, which is run once and shared (default: 1)
+  --logprobs <num>         Print each token's log probability with so many most likely tokens (0 to 32)
   --no-graph               Run every step directly instead of replaying captured CUDA graphs
   --profile                Time each section of the model walk (disables graphs) and print ms per step
   --plain-kernels          Use the plain twin of every kernel
@@ -72,6 +74,8 @@ class CLIOptions:
         self.random_seed: Optional[int] = None
         self.prompt_file: Optional[str] = None
         self.max_slots: Optional[int] = None
+        self.samples = 1
+        self.logprobs: Optional[int] = None
         self.no_graph = False
         self.profile = False
         self.plain_kernels = False
@@ -92,6 +96,7 @@ class CLIOptions:
         "--context-length": ("context_length", int), "-c": ("context_length", int),
         "--dtype": ("dtype", str), "--gpu-device": ("gpu_device", int), "--random": ("random_seed", int),
         "--prompt-file": ("prompt_file", str), "--max-slots": ("max_slots", int),
+        "--samples": ("samples", int), "--logprobs": ("logprobs", int),
     }
     _SWITCHES = {"--no-graph": "no_graph", "--profile": "profile", "--plain-kernels": "plain_kernels"}
     # flags of the reference that place work on devices or threads; accepted, without effect here
@@ -168,6 +173,10 @@ def _print_result(index: int, total: int, response) -> None:
         return
     head = f"[{index}] " if total > 1 else ""
     print(head + " ".join(str(t) for t in response.token_ids))
+    if response.logprobs is not None:
+        for t in response.logprobs:
+            top = "  top " + " ".join(f"{i}:{lp:.4f}" for i, lp in t.top) if t.top else ""
+            print(f"  {t.token_id}  logprob {t.logprob:.4f}  entropy {t.entropy:.4f}  rank {t.rank}{top}")
 
 
 def run(argv: Optional[List[str]] = None) -> int:
@@ -184,7 +193,7 @@ def run(argv: Optional[List[str]] = None) -> int:
     if opts.prompt_file is not None:
         with open(opts.prompt_file) as fh:
             prompts += [parse_ids(line) for line in fh if line.strip()]
-    batch = max(1, len(prompts))
+    batch = max(1, len(prompts), opts.samples)
     engine = Engine.load(opts.model_path, opts.to_engine_options(batch))
     if opts.show_info:
         print(engine.info())
@@ -193,8 +202,14 @@ def run(argv: Optional[List[str]] = None) -> int:
     def generate(prompts: List[List[int]]) -> None:
         print("\n--- Generation ---")
         start = time.perf_counter()
-        responses = engine.generate(prompts, opts.to_sampler_config(), max_tokens=opts.max_tokens,
-                                    stop_token_ids=opts.stop_ids)
+        if opts.samples > 1:                  # several samples of each prompt, which is run once
+            responses = []
+            for p in prompts:
+                responses += engine.generate_samples(p, opts.samples, opts.to_sampler_config(), max_tokens=opts.max_tokens,
+                                                     stop_token_ids=opts.stop_ids, logprobs=opts.logprobs)
+        else:
+            responses = engine.generate(prompts, opts.to_sampler_config(), max_tokens=opts.max_tokens,
+                                        stop_token_ids=opts.stop_ids, logprobs=opts.logprobs)
         elapsed_ms = (time.perf_counter() - start) * 1e3
         for i, r in enumerate(responses):
             _print_result(i, len(responses), r)

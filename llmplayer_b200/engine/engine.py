@@ -44,6 +44,7 @@ class Engine:
                                    kv_dtype=runtime.kv_dtype, device=runtime.device)
         self.workspace = Workspace(runtime.device)
         self._sampler = None
+        self._logprobs = None
         self.last_generation_stats = None
         self.last_step_h2d_bytes = 0
         self.last_step_d2h_bytes = 0
@@ -110,6 +111,11 @@ class Engine:
     def length(self, slot: int) -> int:
         return self.cache.length(slot)
 
+    def fork(self, slot: int, count: int) -> List[int]:
+        """``count`` new slots that go on from where ``slot`` is. They share its full pages, and a step of several of them attends
+        over the shared pages once for all. Each is released by itself."""
+        return self.cache.fork(slot, count)
+
     # ------------------------------------------------------------------ the step
     def plan(self, entries: Sequence[Tuple[int, Sequence[int]]], want: Sequence[Sequence[int]]) -> StepContext:
         """Check a step, reserve its pages and describe it to the device."""
@@ -142,6 +148,7 @@ class Engine:
         counts = [s.num_new for s in sequences]
         self.cache.reserve(slots, counts)
         tables = self.cache.page_tables(slots)
+        shared = self.cache.shared_pages(slots)
         width = 1
         if all(n == 1 for n in counts):
             # steps of one token each are replayed from captured graphs: keep the shape of the
@@ -152,7 +159,10 @@ class Engine:
             width = 8
             while width < longest + 1:
                 width *= 2
-        return StepContext(self.workspace, sequences, tokens, tables, rows, min_table_width=width)
+        elif (self.runtime.device.type == "cuda"
+              and 2 * len(tokens) + sum(len(t) for group in tables for t in group) >= StepContext.ON_DEVICE_ENTRIES):
+            return StepContext(self.workspace, sequences, tokens, tables, rows, shared_pages=shared, on_device=True)
+        return StepContext(self.workspace, sequences, tokens, tables, rows, min_table_width=width, shared_pages=shared)
 
     def run(self, ctx: StepContext) -> torch.Tensor:
         """Run a planned step; returns float32 logits [wanted, vocab] (valid until the next step)."""
@@ -183,14 +193,13 @@ class Engine:
 
     def _run_captured(self, ctx: StepContext, logits: torch.Tensor) -> None:
         """A step of one token per sequence, through a CUDA graph of the model walk for its shape
-        (batch, page-table widths, wanted rows). The first step of a shape runs directly, the
+        (batch, page-table widths and shared pages, wanted rows). The first step of a shape runs directly, the
         second is captured, later ones are replayed; the step's integers were copied to the
         device beforehand, and the graph reads them there (the reference replays its captured
         forward pass the same way: java21 inference/CudaForwardPass.java:1760-1812)."""
         key = ctx.graph_key
         if key is None:
-            key = ctx.graph_key = (ctx.num_sequences, tuple(t.shape[1] for t in ctx.page_tables), ctx.num_wanted,
-                                   ctx.meta.data_ptr())
+            key = ctx.graph_key = (ctx.num_sequences, ctx.table_shapes, ctx.num_wanted, ctx.meta.data_ptr())
         entry = self._graphs.get(key)
         if entry is not None and entry[1] != self.workspace.version:
             entry = None                                  # a buffer moved since the capture
@@ -289,6 +298,26 @@ class Engine:
         self.last_step_h2d_bytes += self._sampler.last_h2d_bytes
         return chosen
 
+    def token_logprobs(self, logits: torch.Tensor, tokens: Sequence[int], *, top: int = 0):
+        """The log probability of one token per row of ``logits``, with the entropy and the ``top`` most likely tokens of each row: a
+        list of :class:`llmplayer_b200.engine.scoring.TokenLogprob`."""
+        if self._logprobs is None:
+            from .scoring import LogprobReader
+            self._logprobs = LogprobReader(self.runtime.device)
+        if self.profiler is not None:
+            ops.set_profiler(self.profiler)
+        try:
+            return self._logprobs.read(logits, tokens, top)
+        finally:
+            ops.set_profiler(None)
+
+    def score(self, prompt: Sequence[int], continuations: Sequence[Sequence[int]], *, top: int = 0):
+        """The log probability of every token of each continuation of ``prompt`` (both token ids), without sampling: one
+        :class:`llmplayer_b200.engine.scoring.ScoredTokens` per continuation, in order. The prompt is run once; the continuations go on
+        from forks of it, as many at a time as the cache has slots and pages for. ``top``: list so many most likely tokens beside each."""
+        from .scoring import score
+        return score(self, prompt, continuations, top)
+
     def decode_steps(self, entries: Sequence[Tuple[int, int]], samplers, *, quiet: Optional[Sequence[int]] = None,
                      stops: Optional[Sequence[Sequence[int]]] = None, max_steps: int = 256) -> List[List[int]]:
         """Decode: feed one token to each sequence (``entries``: ``(slot, token)``), sample each one's next
@@ -351,7 +380,7 @@ class Engine:
         self._last_ctx = ctx
         key = ctx.fused_key
         if key is None:
-            key = ctx.fused_key = (B, tuple(t.shape[1] for t in ctx.page_tables), ctx.meta.data_ptr(), ctx.host_pointer)
+            key = ctx.fused_key = (B, ctx.table_shapes, ctx.meta.data_ptr(), ctx.host_pointer)
         logits = self.workspace.get("logits", (B, self.vocab_size), torch.float32)
         sampled = self.workspace.get("sampled", (B,), torch.int32)
         landing, _ = self.workspace.pinned("sampled_host", B)
@@ -546,8 +575,38 @@ class Engine:
         return (len(token_counts) <= self.cache.slots.num_free
                 and all(need <= free for free in self.cache.free_pages()))
 
+    def forks_fit(self, parent: Optional[int], new_tokens: Sequence[int]) -> bool:
+        """Whether forks of ``parent`` (None: slots of their own) that bring so many tokens each can be held beside what is held now."""
+        have = 0 if parent is None else self.cache.length(parent)
+        need = sum(-(-(have + int(n)) // PAGE_SIZE) - have // PAGE_SIZE for n in new_tokens)
+        return len(new_tokens) <= self.cache.slots.num_free and all(need <= free for free in self.cache.free_pages())
+
+    def generate_samples(self, prompt: Sequence[int], samples: int, sampler_config=None, *, max_tokens: int = 256,
+                         stop_token_ids=None, logprobs: Optional[int] = None):
+        """``samples`` continuations of one prompt, drawn side by side: the prompt is run once, its cached pages are shared, and a decode
+        step attends over them once for all. Sample i draws with the configuration's seed plus i. Returns one
+        :class:`GenerationResponse` per sample."""
+        from ..sampling.params import SamplerConfig
+        from .generate import GenerationLoop, GenerationRequest
+        if int(samples) < 1:
+            raise RequestError(f"{samples} samples of a prompt")
+        config = sampler_config if sampler_config is not None else SamplerConfig()
+        requests = [GenerationRequest(prompt_ids=list(prompt), max_tokens=max_tokens, sampler_config=config.with_seed(config.seed + i),
+                                      stop_token_ids=stop_token_ids, logprobs=logprobs) for i in range(int(samples))]
+        total = min(len(requests[0].prompt_ids) + max(0, max_tokens), self.context_length)
+        shared = len(requests[0].prompt_ids) // PAGE_SIZE
+        need = shared + len(requests) * (-(-total // PAGE_SIZE) - shared)
+        if len(requests) > self.cache.slots.num_free or any(need > free for free in self.cache.free_pages()):
+            raise RequestError(f"the cache cannot hold {samples} samples of {total} tokens on {len(requests[0].prompt_ids)} shared ones")
+        loop = GenerationLoop(self, max_batch=len(requests), context_length=self.context_length,
+                              default_stop_ids=self.config.stop_token_ids())
+        out = loop.run(requests, one_prompt=True)
+        self.last_generation_stats = loop.stats
+        self.check()
+        return out
+
     def generate(self, prompts, sampler_config=None, *, max_tokens: int = 256, stop_token_ids=None,
-                 on_token=None, max_batch: Optional[int] = None, laps=None):
+                 on_token=None, max_batch: Optional[int] = None, laps=None, logprobs: Optional[int] = None):
         """Generate for a batch of prompts (lists of token ids) or of
         :class:`GenerationRequest`; returns one :class:`GenerationResponse` each, in order.
 
@@ -555,7 +614,8 @@ class Engine:
         a prompt, a token budget, sampler options; ``on_token(request_index, token_id)``
         may return False to stop that request. ``stats`` of the last call are kept in
         ``last_generation_stats``; ``laps=(skip, every)`` times the decode steps in laps (see
-        :meth:`GenerationLoop.run`).
+        :meth:`GenerationLoop.run`). ``logprobs=k``: each response lists its tokens' log probabilities with the k most likely
+        tokens beside each (k may be 0); such a batch is decoded one step at a time.
         """
         from ..sampling.params import SamplerConfig
         from .generate import GenerationLoop, GenerationRequest
@@ -567,7 +627,7 @@ class Engine:
                 requests.append(GenerationRequest(
                     prompt_ids=list(p), max_tokens=max_tokens,
                     sampler_config=sampler_config if sampler_config is not None else SamplerConfig(),
-                    stop_token_ids=stop_token_ids))
+                    stop_token_ids=stop_token_ids, logprobs=logprobs))
         loop = GenerationLoop(self, max_batch=max_batch or self.cache.max_slots,
                               context_length=self.context_length,
                               default_stop_ids=self.config.stop_token_ids())

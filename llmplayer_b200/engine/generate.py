@@ -11,7 +11,9 @@ count generated tokens over the time since the prompt was processed (:481, :772-
 
 The loop talks to a *backend* (the engine, or a scripted stand-in in tests):
 ``acquire()``, ``release(slot)``, ``step(entries, want) -> logits``,
-``sample(logits, rows, samplers) -> tokens``, ``fits(token_counts) -> bool``.
+``sample(logits, rows, samplers) -> tokens``, ``fits(token_counts) -> bool``; where
+requests ask for log probabilities ``token_logprobs(logits, tokens, top)``, and for
+several samples of one prompt ``fork(slot, count) -> slots``.
 """
 from __future__ import annotations
 
@@ -30,6 +32,7 @@ class GenerationRequest:
     max_tokens: int = 256
     sampler_config: SamplerConfig = field(default_factory=SamplerConfig)
     stop_token_ids: Optional[Sequence[int]] = None     # None: the model configuration's end tokens
+    logprobs: Optional[int] = None     # report each token's log probability, with so many most likely tokens (None: do not)
 
 
 @dataclass
@@ -41,6 +44,7 @@ class GenerationResponse:
     tokens_per_second: float = 0.0
     time_ms: float = 0.0
     error: Optional[str] = None
+    logprobs: Optional[list] = None    # a TokenLogprob per token, if the request asked for them
 
     @property
     def token_count(self) -> int:
@@ -84,6 +88,7 @@ class _Live:
         self.slot = slot
         self.sampler = SequenceSampler(request.sampler_config)
         self.tokens: List[int] = []
+        self.logprobs: Optional[list] = None if request.logprobs is None else []
         self.next_token: Optional[int] = None
         self.finish: Optional[str] = None
 
@@ -103,8 +108,9 @@ class GenerationLoop:
 
     def run(self, requests: Sequence[GenerationRequest],
             on_token: Optional[Callable[[int, int], Optional[bool]]] = None,
-            laps: Optional[Sequence[int]] = None) -> List[GenerationResponse]:
-        """Generate for every request; responses come in request order.
+            laps: Optional[Sequence[int]] = None, one_prompt: bool = False) -> List[GenerationResponse]:
+        """Generate for every request; responses come in request order. ``one_prompt``: all requests have the same prompt, which is
+        run once and forked (the backend's ``fork``); the caller has made sure that they fit the cache together.
 
         ``laps = (skip, every)``: for measurements. After the first ``skip`` decode steps of a batch, the
         decode steps are timed in laps of ``every`` steps each; ``stats.laps`` gets one entry per full lap:
@@ -123,7 +129,7 @@ class GenerationLoop:
                     error=f"Error: prompt too long ({n} tokens, max {self.context_length - 1})")
             elif req.max_tokens <= 0:
                 responses[i] = GenerationResponse([], n, "length")
-            elif not self.backend.fits([self._need(req)]):
+            elif not one_prompt and not self.backend.fits([self._need(req)]):
                 responses[i] = GenerationResponse(
                     [], n, "error", error=f"Error: the cache cannot hold {self._need(req)} tokens for this request")
             else:
@@ -133,11 +139,11 @@ class GenerationLoop:
             needs: List[int] = []
             while pending and len(batch) < self.max_batch:
                 need = self._need(requests[pending[0]])
-                if batch and not self.backend.fits(needs + [need]):
+                if batch and not one_prompt and not self.backend.fits(needs + [need]):
                     break
                 batch.append(pending.pop(0))
                 needs.append(need)
-            self._run_batch(batch, requests, responses, on_token)
+            self._run_batch(batch, requests, responses, on_token, one_prompt)
         return responses  # type: ignore[return-value]
 
     # ------------------------------------------------------------------ one batch
@@ -147,6 +153,8 @@ class GenerationLoop:
             s.finish = "stop"
             return
         s.tokens.append(tok)
+        if s.logprobs is not None:
+            s.logprobs.append(s.scored)
         self.stats.generated_tokens += 1
         if on_token is not None and on_token(s.index, tok) is False:
             s.finish = "callback"
@@ -166,13 +174,27 @@ class GenerationLoop:
         by_budget = s.request.max_tokens - len(s.tokens) - 1
         return max(0, min(by_context, by_budget))
 
-    def _run_batch(self, batch, requests, responses, on_token) -> None:
+    def _choose(self, live: List[_Live], logits, rows: List[int]) -> List[int]:
+        """One token for each sequence from its row of the logits, and its log probability where the request asks for it."""
+        chosen = self.backend.sample(logits, rows, [s.sampler for s in live])
+        wanted = [s.request.logprobs for s in live if s.logprobs is not None]
+        if wanted:
+            if rows != list(range(len(live))):
+                logits = logits[rows]
+            scored = self.backend.token_logprobs(logits[:len(live)], [int(t) for t in chosen], top=max(wanted))
+            for s, t in zip(live, scored):
+                if s.logprobs is not None:
+                    t.top = t.top[:s.request.logprobs]
+                    s.scored = t
+        return chosen
+
+    def _run_batch(self, batch, requests, responses, on_token, one_prompt: bool = False) -> None:
         be = self.backend
         live: List[_Live] = []
         for i in batch:
             req = requests[i]
             stop = self.default_stop_ids if req.stop_token_ids is None else tuple(req.stop_token_ids)
-            live.append(_Live(i, req, frozenset(int(t) for t in stop), be.acquire()))
+            live.append(_Live(i, req, frozenset(int(t) for t in stop), be.acquire() if not (one_prompt and live) else None))
         self.stats.batches += 1
         several = getattr(be, "decode_steps", None)       # a backend that can run several quiet steps per call
         mark = getattr(be, "mark", None)
@@ -182,15 +204,19 @@ class GenerationLoop:
         t_decode = None
         started = None
         try:
-            logits = be.step([(s.slot, list(s.request.prompt_ids)) for s in live],
-                             [[len(s.request.prompt_ids) - 1] for s in live])
-            pending = [be.sample(logits, list(range(len(live))), [s.sampler for s in live])]
+            run = live[:1] if one_prompt else live
+            logits = be.step([(s.slot, list(s.request.prompt_ids)) for s in run],
+                             [[len(s.request.prompt_ids) - 1] for s in run])
+            if one_prompt and len(live) > 1:
+                for s, slot in zip(live[1:], be.fork(live[0].slot, len(live) - 1)):
+                    s.slot = slot
+            pending = [self._choose(live, logits, [0] * len(live) if one_prompt else list(range(len(live))))]
             # the prompt is processed once its logits are there: decode time starts here
             t_decode = time.perf_counter()
             started = mark() if mark is not None else None
             launched = count() if count is not None else None
             self.stats.prefill_ms += (t_decode - t0) * 1e3
-            self.stats.prompt_tokens += sum(len(s.request.prompt_ids) for s in live)
+            self.stats.prompt_tokens += sum(len(s.request.prompt_ids) for s in run)
             step_index = 0
             steps_done = 0
             boundary = None                       # the decode step count at which the current lap ends
@@ -213,20 +239,20 @@ class GenerationLoop:
                         responses[s.index] = GenerationResponse(
                             s.tokens, len(s.request.prompt_ids), s.finish,
                             tokens_per_second=len(s.tokens) / elapsed if elapsed > 0 and s.tokens else 0.0,
-                            time_ms=(now - t0) * 1e3)
+                            time_ms=(now - t0) * 1e3, logprobs=s.logprobs)
                         be.release(s.slot)
                         s.slot = None
                 live = [s for s in live if s.finish is None]
                 if not live:
                     break
-                if several is not None:
+                if several is not None and all(s.logprobs is None for s in live):
                     quiet = [0 if on_token is not None else self._quiet(s, step_index) for s in live]
                     most = 256 if boundary is None else max(1, min(256, boundary - steps_done))
                     pending = several([(s.slot, s.next_token) for s in live], [s.sampler for s in live],
                                       quiet=quiet, stops=[s.stop_ids for s in live], max_steps=most)
                 else:
                     logits = be.step([(s.slot, [s.next_token]) for s in live], [[0] for _ in live])
-                    pending = [be.sample(logits, list(range(len(live))), [s.sampler for s in live])]
+                    pending = [self._choose(live, logits, list(range(len(live))))]
                 self.stats.decode_steps += len(pending)
                 self.stats.step_tokens += len(live) * len(pending)
                 steps_done += len(pending)

@@ -15,6 +15,8 @@ from typing import Dict, List, Optional, Sequence, Tuple
 
 import torch
 
+from ..cache.pages import PAGE_SIZE
+
 
 @dataclass(frozen=True)
 class SequenceStep:
@@ -133,11 +135,20 @@ class StepContext:
 
     A context of one token per sequence can be moved on to the next step of the same sequences
     (:meth:`advance`): only the tokens, positions and lengths are copied again.
+
+    ``shared_pages`` per cache group: so many first columns of its page table are the same in every row. ``on_device``: only
+    tokens, lengths and the pages' numbers are copied, shared ones once, and a kernel builds the tables from them
+    (``ops.step_tables``); such a context cannot be moved on.
     """
+
+    # From so many entries of the tables on they are built on the device. On the host an entry costs about 50 ns, the kernel's launch
+    # about 15 us for each cache group.
+    ON_DEVICE_ENTRIES = 1024
 
     def __init__(self, workspace: Workspace, sequences: List[SequenceStep], tokens: Sequence[int],
                  page_tables: List[List[List[int]]], wanted_rows: Sequence[int], *,
-                 min_table_width: int = 1, meta_name: str = "step_meta"):
+                 min_table_width: int = 1, meta_name: str = "step_meta", shared_pages: Optional[Sequence[int]] = None,
+                 on_device: bool = False):
         self.workspace = workspace
         self._sequences: Optional[List[SequenceStep]] = sequences
         self.slot_list = [s.slot for s in sequences]
@@ -152,6 +163,11 @@ class StepContext:
         self.wanted_rows = list(wanted_rows)
         # one token for each sequence and every sequence's logits wanted: the shape a decode step continues in
         self.continues_all = self.all_single and self.wanted_rows == list(range(B))
+        self.shared_pages = list(shared_pages) if shared_pages is not None else [0] * len(page_tables)
+        if on_device:
+            self.continues_all = False
+            self._build_on_device(sequences, tokens, page_tables, meta_name)
+            return
 
         widths = [max([min_table_width] + [len(t) for t in group]) for group in page_tables]
         self._widths = widths
@@ -201,6 +217,46 @@ class StepContext:
         self.q_start = meta[o[5]:o[5] + B + 1]
         self.page_tables = [meta[o[6 + g]:o[6 + g] + B * w].view(B, w) for g, w in enumerate(widths)]
         self.rows = meta[o[-1]:o[-1] + W]
+
+    def _build_on_device(self, sequences: List[SequenceStep], tokens: Sequence[int], page_tables: List[List[List[int]]],
+                         meta_name: str) -> None:
+        from ..kernels import ops
+        T, B, W = self.num_tokens, self.num_sequences, self.num_wanted
+        blocks = [-(-(s.first_position + s.num_new) // PAGE_SIZE) for s in sequences]
+        shared = [group[0][:n] for group, n in zip(page_tables, self.shared_pages)]
+        own = [[page for table, k in zip(group, blocks) for page in table[n:k]] for group, n in zip(page_tables, self.shared_pages)]
+        arrays = [tokens, self.slot_list, self.first_positions, self.new_counts, self.wanted_rows]
+        for pair in zip(shared, own):
+            arrays.extend(pair)
+        offsets, total = [], 0
+        for values in arrays:
+            offsets.append(total)
+            total += _round_up(max(len(values), 1), 4)            # keep every array 16-byte aligned
+        host, self._copied = self.workspace.pinned(meta_name, total)
+        self._host, self._view = host, host.numpy()
+        for o, values in zip(offsets, arrays):
+            self._view[o:o + len(values)] = values
+        self.meta = meta = self.workspace.get(meta_name, (total,), torch.int32)
+        self._total, self._moving, self._upload_views, self._pinned = total, total, {}, host.is_pinned()
+        self.graph_key = self.fused_key = None
+        self._upload(total)
+        parts = [meta[o:o + len(values)] for o, values in zip(offsets, arrays)]
+        self.tokens, self.slots, first, count, self.rows = parts[:5]
+        get = self.workspace.get
+        self.positions, self.seq_ids = get("step_positions", (T,), torch.int32), get("step_seq_ids", (T,), torch.int32)
+        self.kv_len, self.q_start = get("step_kv_len", (B,), torch.int32), get("step_q_start", (B + 1,), torch.int32)
+        width = max(max(blocks), 1)
+        self.page_tables = []
+        for g in range(len(page_tables)):
+            table = get(f"step_page_table{g}", (B, width), torch.int32)
+            described = (self.q_start, self.kv_len, self.positions, self.seq_ids) if g == 0 else (None,) * 4
+            ops.step_tables(first, count, parts[5 + 2 * g], parts[6 + 2 * g], *described, table, page_size=PAGE_SIZE)
+            self.page_tables.append(table)
+
+    @property
+    def table_shapes(self) -> tuple:
+        """What a captured graph of the step depends on of its page tables: (width, shared pages) per cache group."""
+        return tuple((t.shape[1], n) for t, n in zip(self.page_tables, self.shared_pages))
 
     @property
     def sequences(self) -> List[SequenceStep]:

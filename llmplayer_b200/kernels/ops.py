@@ -1246,13 +1246,20 @@ def attention_decode_fused(qkv: torch.Tensor, rotation: Rotation, out: torch.Ten
 def attention(ctx, q: torch.Tensor, out: torch.Tensor, pages: torch.Tensor, page_table: torch.Tensor, *,
               num_heads: int, num_kv_heads: int, head_dim: int, scale: float, window: Optional[int],
               fast: bool, softcap: Optional[float] = None, sinks: Optional[torch.Tensor] = None,
-              exact_weights: bool = False, keep_first: int = 0, chunk: int = 0, distance=None, gate=None) -> torch.Tensor:
+              exact_weights: bool = False, keep_first: int = 0, chunk: int = 0, distance=None, gate=None,
+              shared_pages: int = 0) -> torch.Tensor:
     """Attention of the step's tokens over the cache; picks the kernel for the step's shape. ``keep_first`` (with a
     window): the first tokens of a sequence that stay visible beyond the window. ``chunk``, ``distance``,
-    ``gate``: see :func:`attention_plain`."""
+    ``gate``: see :func:`attention_plain`. ``shared_pages``: so many first columns of the page table are the same in every row
+    (see :func:`attention_shared`; used where nothing shapes the scores and the kernel is built for the heads)."""
     tensor_cores = (fast and q.dtype == torch.bfloat16 and pages.dtype == torch.bfloat16
                     and head_dim % 16 == 0 and head_dim <= 256)
     keep_first = int(keep_first) if window else 0
+    if (tensor_cores and shared_pages and not window and not softcap and sinks is None and not exact_weights and not chunk
+            and distance is None and gate is None and attention_shared_serves(num_heads, num_kv_heads, head_dim, pages.shape[3])
+            and attention_shared_pays(page_table.shape[0], shared_pages, ctx.all_single)):
+        return attention_shared(q, out, pages, page_table, ctx.q_start, ctx.kv_len, ctx.buffer, shared_pages=shared_pages,
+                                max_new=ctx.max_new, num_heads=num_heads, num_kv_heads=num_kv_heads, head_dim=head_dim, scale=scale)
     if tensor_cores and ctx.all_single:
         return attention_decode(q, out, pages, page_table, ctx.kv_len, ctx.buffer, num_heads=num_heads,
                                 num_kv_heads=num_kv_heads, head_dim=head_dim, scale=scale, window=window,
@@ -1273,6 +1280,17 @@ def attention_shared_serves(num_heads: int, num_kv_heads: int, head_dim: int, pa
     """Whether :func:`attention_shared` is built for these heads."""
     return (head_dim in (64, 128) and page_size == 64 and num_kv_heads > 0 and num_heads % num_kv_heads == 0
             and num_heads // num_kv_heads <= 128)
+
+
+# From how many pages read over again (sequences times shared pages) on the shared form is used: 256 for a step of single tokens, whose
+# other form rotates, stores and attends in one kernel, 64 for several tokens. B200, 32 heads on 8, shared against ordinary attention alone:
+# single tokens, heads of 64: 8 sequences on 32 pages 18.4 against 26.6 us, on 16 pages 14.3 against 18.4; 64 on 4 14.3 against 16.4;
+# 24 tokens each: 2 sequences on 32 pages 24.6 against 41 us, on 16 22.5 against 24.5; 8 on 8 18.4 against 20.4, on 4 18.4 against 16.4.
+SHARED_PAGES_SINGLE, SHARED_PAGES_SEVERAL = 256, 64
+
+
+def attention_shared_pays(sequences: int, shared_pages: int, single: bool) -> bool:
+    return sequences > 1 and sequences * shared_pages >= (SHARED_PAGES_SINGLE if single else SHARED_PAGES_SEVERAL)
 
 
 def attention_shared(q: torch.Tensor, out: torch.Tensor, pages: torch.Tensor, page_table: torch.Tensor, q_start: torch.Tensor,

@@ -149,6 +149,14 @@ class Attention(Part):
                          int(s.keep_first or 0), s.chunk)
 
     # ------------------------------------------------------------------ step
+    def _shared_pages(self, ctx, cache) -> int:
+        """How many of the cache group's first pages all of the step's sequences share, if it pays to attend over them once."""
+        s = self.spec
+        n = ctx.shared_pages[cache.group_index]
+        serves = (n > 0 and self.runtime.fast and s.window is None and s.chunk is None and cache.pages.dtype == torch.bfloat16
+                  and ops.attention_shared_serves(s.num_heads, s.num_kv_heads, s.head_dim, cache.pages.shape[3]))
+        return n if serves and ops.attention_shared_pays(ctx.num_sequences, n, ctx.all_single) else 0
+
     @property
     def offers_inputs(self) -> bool:
         """Whether an owner may form this part's input projections in a wider product (the general path only)."""
@@ -236,7 +244,8 @@ class Attention(Part):
         with ops.section("attention.scores"):
             ops.attention(ctx, q, o, cache.pages, table, num_heads=H, num_kv_heads=G, head_dim=hd, scale=s.scale,
                           window=s.window, fast=rt.fast, softcap=s.softcap, sinks=self.sinks, exact_weights=s.exact_weights,
-                          keep_first=int(s.keep_first or 0), chunk=int(s.chunk or 0), distance=self.distance, gate=gate)
+                          keep_first=int(s.keep_first or 0), chunk=int(s.chunk or 0), distance=self.distance, gate=gate,
+                          shared_pages=ctx.shared_pages[cache.group_index])
         with ops.section("attention.out"):
             if overwrite:
                 if clear is not None:
@@ -266,9 +275,11 @@ class Attention(Part):
         # the position encoding as something the kernels do on the way (a rotation), or None: then the
         # encoding's own part changes queries and keys in the projection's output before the kernels run
         rotation = self.position.rotation()
+        # a batch whose sequences begin with the same pages: those are attended over once for all, by kernels of their own
+        shared = self._shared_pages(ctx, cache)
         if isinstance(x, PendingNorm):
             T = residual.shape[0]
-            if (rt.fast and ctx.all_single and x.fusable and cache.pages.dtype == torch.bfloat16 and hd % 16 == 0
+            if (rt.fast and not shared and ctx.all_single and x.fusable and cache.pages.dtype == torch.bfloat16 and hd % 16 == 0
                     and hd <= 256 and self.qkv.can_few(T, ops.STORE) and self.out.can_few(T, ops.ACCUMULATE)
                     and residual.dtype == torch.float32 and rotation is not None):
                 self._forward_few(ctx, cache, x, residual, rotation)
@@ -288,7 +299,7 @@ class Attention(Part):
                                   None if s.shares_kv else cache.pages, num_heads=H, num_kv_heads=G, head_dim=hd)
             with ops.section("attention.scores"):
                 ops.attention(ctx, q, o, cache.pages, table, num_heads=H, num_kv_heads=G, head_dim=hd,
-                              scale=s.scale, window=s.window, fast=True)
+                              scale=s.scale, window=s.window, fast=True, shared_pages=shared)
             with ops.section("attention.out"):
                 return self.out.accumulate(o, residual, ctx, then_norm)
         qkv = ctx.buffer("qkv", (T, self.qkv.out_features), torch.float32)
@@ -298,7 +309,7 @@ class Attention(Part):
             with ops.section("attention.position"):
                 self.position.apply(ctx, qkv, num_heads=H, num_kv_heads=0 if s.shares_kv else G, head_dim=hd)
             rotation = ops.NO_ROTATION
-        if rt.fast and ctx.all_single and cache.pages.dtype == torch.bfloat16 and hd % 16 == 0 and hd <= 256:
+        if rt.fast and not shared and ctx.all_single and cache.pages.dtype == torch.bfloat16 and hd % 16 == 0 and hd <= 256:
             # one token per sequence: rotation, cache write, attention and the merge of its shares in one kernel
             with ops.section("attention.scores"):
                 ops.attention_decode_fused(
@@ -315,7 +326,7 @@ class Attention(Part):
                 num_heads=H, num_kv_heads=G, head_dim=hd)
         with ops.section("attention.scores"):
             ops.attention(ctx, q, o, cache.pages, table, num_heads=H, num_kv_heads=G, head_dim=hd,
-                          scale=s.scale, window=s.window, fast=rt.fast)
+                          scale=s.scale, window=s.window, fast=rt.fast, shared_pages=shared)
         with ops.section("attention.out"):
             return self.out.accumulate(o, residual, ctx, then_norm)
 
