@@ -144,7 +144,7 @@ _SIGNATURES = {
     "step_tables": {
         "lp_step_tables": [_P, _P, _P, _I, _P, _I, _P, _P, _P, _P, _I, _P, _I, _I, _I, _P],
         "lp_copy_pages_most": [],
-        "lp_copy_pages": [_P, _I, ctypes.c_longlong, ctypes.c_longlong, _P, _P, _I, _P],
+        "lp_copy_pages": [_P, _I, ctypes.c_longlong, ctypes.c_longlong, _P, _I, _P],
     },
     "attention_shared": {
         "lp_attention_shared": [_P, _P, _P, ctypes.c_longlong, _P, _I, _P, _P, _I, _I, _I, _I, _I, _I, _I, _F, _I, _P, _P, _P, _P],
@@ -423,6 +423,22 @@ def _on_current_device(what: str, *tensors: Optional[torch.Tensor]) -> None:
     for t in tensors:
         if t is not None and t.get_device() != device:
             raise KernelError(f"{what}: a tensor on {t.device}, the current device is cuda:{device}")
+
+
+def _want_all(what: str, names: str, dtype, ndim: int, *tensors: torch.Tensor) -> None:
+    """:func:`_want` and :func:`_on_current_device` for several tensors of one kind; ``names``: theirs, in order."""
+    device = torch._C._cuda_getDevice()
+    try:
+        for t in tensors:
+            if t.get_device() != device or t.dtype is not dtype or t.dim() != ndim or not t.is_contiguous():
+                break
+        else:
+            return
+    except AttributeError:
+        pass
+    for t, name in zip(tensors, names.split()):
+        _want(t, f"{what} {name}", dtype, ndim)
+        _on_current_device(what, t)
 
 
 # --------------------------------------------------------------------------- embedding
@@ -1306,9 +1322,8 @@ def attention_shared(q: torch.Tensor, out: torch.Tensor, pages: torch.Tensor, pa
     matter, and those of ``out`` stay as they are. ``scratch(name, shape, dtype)`` supplies buffers for partial results."""
     what = "attention_shared"
     _check_attention(q, out, pages, page_table, num_heads, num_kv_heads, head_dim, what)
-    _want(q_start, f"{what} q_start", torch.int32, 1)
-    _want(kv_len, f"{what} kv_len", torch.int32, 1)
-    _on_current_device(what, q, out, pages, page_table, q_start, kv_len)
+    _want_all(what, "q_start kv_len", torch.int32, 1, q_start, kv_len)
+    _on_current_device(what, q, out, pages, page_table)
     B, T = kv_len.numel(), q.shape[0]
     if B == 0 or q_start.numel() != B + 1 or page_table.shape[0] != B:
         raise KernelError(f"{what}: {B} sequences, {q_start.numel()} offsets, table {tuple(page_table.shape)}")
@@ -1365,61 +1380,59 @@ def step_tables(first: torch.Tensor, count: torch.Tensor, shared: torch.Tensor, 
     Entries of the latter two behind the last sequence's tokens stay as they are. Nothing is written beyond the
     tensors' sizes and nothing read beyond ``own``, whatever the lengths say."""
     what = "step_tables"
-    for t, name in ((first, "first"), (count, "count"), (shared, "shared"), (own, "own")):
-        _want(t, f"{what} {name}", torch.int32, 1)
-    _want(page_table, f"{what} page_table", torch.int32, 2)
-    B = first.numel()
-    if B == 0 or count.numel() != B or page_table.shape[0] != B or page_table.shape[1] == 0:
+    rest = (q_start, kv_len, positions, seq_ids)
+    if q_start is None or kv_len is None or positions is None or seq_ids is None:
+        if any(t is not None for t in rest):
+            raise KernelError(f"{what}: q_start, kv_len, positions and seq_ids go together")
+        _want_all(what, "first count shared own", torch.int32, 1, first, count, shared, own)
+        tokens = 0
+    else:
+        _want_all(what, "first count shared own q_start kv_len positions seq_ids", torch.int32, 1, first, count, shared, own, *rest)
+        tokens = positions.numel()
+    _want_all(what, "page_table", torch.int32, 2, page_table)
+    B, (rows, width) = first.numel(), page_table.shape
+    if B == 0 or count.numel() != B or rows != B or width == 0:
         raise KernelError(f"{what}: {B} sequences, {count.numel()} counts, table {tuple(page_table.shape)}")
     if int(page_size) < 1:
         raise KernelError(f"{what}: pages of {page_size} positions")
-    rest = (q_start, kv_len, positions, seq_ids)
-    if any(t is None for t in rest) != all(t is None for t in rest):
-        raise KernelError(f"{what}: q_start, kv_len, positions and seq_ids go together")
-    tokens = 0
-    if q_start is not None:
-        for t, name in zip(rest, ("q_start", "kv_len", "positions", "seq_ids")):
-            _want(t, f"{what} {name}", torch.int32, 1)
-        tokens = positions.numel()
-        if q_start.numel() != B + 1 or kv_len.numel() != B or seq_ids.numel() != tokens:
-            raise KernelError(f"{what}: {B} sequences, {q_start.numel()} offsets, {kv_len.numel()} lengths, {tokens} positions of "
-                              f"{seq_ids.numel()} tokens")
-    _on_current_device(what, first, count, shared, own, page_table, *rest)
+    if q_start is not None and (q_start.numel() != B + 1 or kv_len.numel() != B or seq_ids.numel() != tokens):
+        raise KernelError(f"{what}: {B} sequences, {q_start.numel()} offsets, {kv_len.numel()} lengths, {tokens} positions of "
+                          f"{seq_ids.numel()} tokens")
     lib = library("step_tables")
     _check(lib, lib.lp_step_tables(first.data_ptr(), count.data_ptr(), shared.data_ptr(), shared.numel(), own.data_ptr(), own.numel(),
                                    _ptr(q_start), _ptr(kv_len), _ptr(positions), _ptr(seq_ids), tokens, page_table.data_ptr(),
-                                   page_table.shape[1], B, int(page_size), _stream()))
+                                   width, B, int(page_size), _stream()))
 
 
 def copy_pages(storage: torch.Tensor, sources, targets) -> None:
     """Copy pages of a cache group's ``storage`` [runs, num_pages, ...] in every run: page ``sources[i]`` to page ``targets[i]``
     (numbers on the host). A page may be copied to several others; no page is a target twice or a target and a source."""
     what = "copy_pages"
-    sources, targets = [int(p) for p in sources], [int(p) for p in targets]
+    sources, targets = list(map(int, sources)), list(map(int, targets))
     if len(sources) != len(targets):
         raise KernelError(f"{what}: {len(sources)} sources and {len(targets)} targets")
     if not isinstance(storage, torch.Tensor) or storage.dim() < 3:
         raise KernelError(f"{what}: expected a storage tensor [runs, pages, ...]")
-    num_pages = storage.shape[1]
-    for p in sources + targets:
-        if not 0 <= p < num_pages:
-            raise KernelError(f"{what}: page {p} of {num_pages}")
-    if len(set(targets)) != len(targets) or not set(targets).isdisjoint(sources):
+    runs, num_pages = storage.shape[:2]
+    if targets and not (0 <= min(sources) and max(sources) < num_pages and 0 <= min(targets) and max(targets) < num_pages):
+        raise KernelError(f"{what}: pages {sources} to {targets} of {num_pages}")
+    distinct = set(targets)
+    if len(distinct) != len(targets) or not distinct.isdisjoint(sources):
         raise KernelError(f"{what}: a page is a target twice, or a target and a source")
     _want(storage, f"{what} storage")
     _on_current_device(what, storage)
-    page_bytes = storage[0, 0].numel() * storage.element_size() if storage.numel() else 0
-    if not targets or page_bytes == 0:
+    elements = storage.numel()
+    if not targets or elements == 0:
         return
+    page_bytes = elements // (runs * num_pages) * storage.element_size()
     if page_bytes % 16 or storage.data_ptr() % 16:
         raise KernelError(f"{what}: pages of {page_bytes} bytes at {storage.data_ptr():#x}: they must be whole vectors of 16 bytes")
     lib = library("step_tables")
     most = lib.lp_copy_pages_most()
     for a in range(0, len(targets), most):
         n = min(most, len(targets) - a)
-        pairs = ctypes.c_int * n
-        _check(lib, lib.lp_copy_pages(storage.data_ptr(), storage.shape[0], num_pages, page_bytes, pairs(*sources[a:a + n]),
-                                      pairs(*targets[a:a + n]), n, _stream()))
+        pairs = (ctypes.c_int * (2 * n))(*sources[a:a + n], *targets[a:a + n])
+        _check(lib, lib.lp_copy_pages(storage.data_ptr(), runs, num_pages, page_bytes, pairs, n, _stream()))
 
 
 # --------------------------------------------------------------------------- latent attention
@@ -2726,16 +2739,15 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, logprob: torch.T
         raise KernelError(f"{what} logits: expected rows of consecutive values, got shape {tuple(logits.shape)}, strides {logits.stride()}")
     code = _code(logits, f"{what} logits")
     R, V = logits.shape
-    _want(targets, f"{what} targets", torch.int32, 1)
-    _want(logprob, f"{what} logprob", torch.float32, 1)
-    _want(entropy, f"{what} entropy", torch.float32, 1)
-    _want(rank, f"{what} rank", torch.int32, 1)
+    _on_current_device(what, logits)
+    _want_all(what, "targets rank", torch.int32, 1, targets, rank)
+    _want_all(what, "logprob entropy", torch.float32, 1, logprob, entropy)
     top = 0
     if (top_ids is None) != (top_logprobs is None):
         raise KernelError(f"{what}: top_ids and top_logprobs go together")
     if top_ids is not None:
-        _want(top_ids, f"{what} top_ids", torch.int32, 2)
-        _want(top_logprobs, f"{what} top_logprobs", torch.float32, 2)
+        _want_all(what, "top_ids", torch.int32, 2, top_ids)
+        _want_all(what, "top_logprobs", torch.float32, 2, top_logprobs)
         top = top_ids.shape[1]
         if top_ids.shape != (R, top) or top_logprobs.shape != (R, top):
             raise KernelError(f"{what}: top_ids {tuple(top_ids.shape)}, top_logprobs {tuple(top_logprobs.shape)} for {R} rows")
@@ -2743,7 +2755,6 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, logprob: torch.T
         raise KernelError(f"{what}: {R} rows, {targets.numel()} targets, outputs of {logprob.numel()}, {entropy.numel()}, {rank.numel()}")
     if V == 0 or top > min(V, TOP_LOGPROBS_MOST):
         raise KernelError(f"{what}: the {top} most likely of {V} tokens (at most {TOP_LOGPROBS_MOST})")
-    _on_current_device(what, logits, targets, logprob, entropy, rank, top_ids, top_logprobs)
     if R == 0:
         return
     lib = library("scoring")
