@@ -8,7 +8,15 @@
 //                  (token, query head) pairs, and neither the products nor the softmax knows sequences. With 64 sequences and 4 query heads
 //                  per key head that is 256 rows on one read of the keys, instead of 64 reads. Tensor memory, tcgen05.
 //   own pages      One kernel per step form (a single token per sequence, several tokens) takes the sequence's own pages with
-//                  mma.sync, then joins its result with what the first kernel left in float32. It starts under the first kernel's tail.
+//                  mma.sync, then joins its result with what the first kernel left in float32. Its reads of its own pages
+//                  begin before the first kernel's results are there (programmatic launch), as far as the SMs have room.
+//
+// B200, 32 query heads on 8, caches cold, the whole call in a graph, against attention that reads every sequence's pages:
+//   64 single tokens, heads of 128, 128 shared pages, up to 250 own positions each: 39 us against 432; the two kernels by
+//       themselves 21 and 15 us for 70 MB (10.8 us at the measured copy rate).
+//   24 sequences of 9 to 37 tokens, heads of 64, 50 shared pages: 45 against 234; 34 and 13 us for 15 GFLOP.
+//   40 sequences of 47 to 190 tokens, heads of 128, 500 shared pages: 2,090 against 5,390; 2,050 and 99 us, 1,175 TFLOP/s, 72 % of
+//       the measured rate of dense products; 2,370 over a long run, where the power limit holds the clock down.
 //
 // All sums, maxima and partial results are float32. The softmax weights enter the products with the values as bfloat16, rounded
 // against a reference maximum (as in the other attention kernels here); the row sums use the float32 weights.
@@ -29,9 +37,13 @@ constexpr float RESCALE_ABOVE = 8.0f;     // log2: how far a row's reference max
 // alternate pages (their results are two partial ones). Per page and chain:
 //   S[128 x 64] = Q K^T (tensor memory)  ->  a thread per row: maximum, exp2, sum, weights as bfloat16 over S in tensor memory
 //   ->  O[128 x HD] += P V (P from tensor memory, V from shared memory, contiguous in N).
-// A chain has two S tiles: the scores of its next page are there when it has finished with one, so a chain never waits for
-// the tensor cores. (With one tile of 128 keys per chain it did, and the two chains' softmaxes ran one behind the other: 4,000 cycles per
-// 128 keys at heads of 128, 2,370 us for 40 x 190 tokens over 500 shared pages, 32 heads on 8.)
+// A chain has two S tiles: the scores of its next page are asked for before it has finished with one. (With one tile of 128 keys
+// per chain the two chains' softmaxes ran one behind the other: 4,000 cycles per 128 keys at heads of 128.)
+// What bounds it: a page of 64 keys takes 1,700 to 2,000 cycles for both chains. The products alone take 1,650 of them (two of
+// 128 x 64 x 128 each way), the softmaxes alone 1,760 (1,024 of those are the exp2 unit's: 2 x 128 x 64 at 16 per cycle). At the 500
+// pages above these took longer than the 2,020 to 2,090 us: a fixed order between the chains 2,386, two groups of softmax warps per chain
+// 2,061, blocks of 128 keys on two threads per row 2,526, weights in tiles of their own and scores given back early 2,150; a polynomial
+// for part of the exponentials gave less than 2 %.
 template <int HD> struct Shape {
     static constexpr int BLOCKS = HD / 64;                          // blocks of 64 features (one swizzle row each)
     static constexpr int TILE = PAGE * HD * 2;                      // keys or values of a page
@@ -99,6 +111,8 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 }
 
 struct SharedArgs {
+    const __nv_bfloat16* kv;     // [num_pages, 2, G, PAGE, HD]
+    long long num_pages;
     const int* table;            // the first row of the page table: its first `pages` entries are the shared pages
     const int* q_start;          // [B + 1]
     const int* kv_len;           // [B]
@@ -183,6 +197,7 @@ attention_shared_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
         // begin with a round trip to memory.
         int held = lane < n ? a.table[first + lane] : 0, before = 0, loaded = 32;
         int at[2] = {0, 0};                                        // tiles asked for, per stream
+        int reached = 0;                                           // the greatest length
         bool ok = true;
         auto request = [&](int k, int c, int which) {
             const int i = page_of(k, c);
@@ -195,7 +210,20 @@ attention_shared_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
             const int s = slot_of(at[c], c);
             ok = __all_sync(0xffffffffu, mbar_wait(&empty[s], round_of(at[c]) ^ 1));
             if (!ok) { if (lane == 0) atomicExch(a.status, 81); return; }
-            if (lane == 0) {
+            const int filled = which ? reached - (first + i) * PAGE : PAGE;
+            if (filled < PAGE) {
+                // Behind the longest sequence values may be no numbers, and no weight of zero takes them out: the page is brought in by hand.
+                const __nv_bfloat16* from = a.kv + ((long long)(page * 2ll + 1) * a.G + g) * (PAGE * HD);
+                for (int x = lane; x < PAGE * (HD / 8); x += 32) {
+                    const int r = x / (HD / 8), chunk = x % (HD / 8);
+                    const bool there = r < filled && page >= 0 && page < a.num_pages;
+                    *reinterpret_cast<uint4*>(ring + s * TILE + tile_offset<true>(r, chunk, HD, HD / 8)) =
+                        there ? *reinterpret_cast<const uint4*>(from + r * HD + chunk * 8) : make_uint4(0, 0, 0, 0);
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&full[s]);
+            } else if (lane == 0) {
                 mbar_expect_tx(&full[s], (uint32_t)TILE);
                 const int row = ((page * 2 + which) * a.G + g) * PAGE;
 #pragma unroll
@@ -208,6 +236,9 @@ attention_shared_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
 #pragma unroll
             for (int c = 0; c < 2; ++c)
                 if (ok && k < counts[c]) request(k, c, 0);
+        for (int b = lane; b < a.B; b += 32) reached = max(reached, a.kv_len[b]);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) reached = max(reached, __shfl_xor_sync(0xffffffffu, reached, o));
         for (int k = 0; k < counts[0] && ok; ++k)                  // the first stream has as many pages as the second, or one more
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
@@ -432,6 +463,8 @@ __device__ __forceinline__ void clear_values(uint8_t* v_tile, int from, int to, 
 // A single new token per sequence: the keys are the rows of the products and the (up to 8) query heads of a key/value head their
 // columns (see attention_decode.cuh); four warps share a page, 16 keys each. grid: (G x head groups, B); 128 threads. Keys and values of a
 // page come one by one through a ring of three tiles (two pages at heads of 64), so that four CTAs share an SM at heads of 128.
+// Bound by the latency of a page's way (number, tiles, products) and of the join at one or two rounds of pages per CTA: 15 us for the 64
+// sequences above, whose own pages are 37 MB (5.6 us), with 17 MB of results that mostly come from L2.
 template <int HD> struct OwnShape {
     static constexpr int TILE = PAGE * HD * 2;
     static constexpr int TILES = HD == 64 ? 4 : 3;
@@ -636,7 +669,9 @@ attention_own_single_kernel(const __grid_constant__ CUtensorMap map_kv, const Ow
     }
 }
 
-// Several new tokens: 64 rows of (token, query head) pairs of one sequence, 16 per warp, over its own pages, causal.
+// Several new tokens: 64 rows of (token, query head) pairs of one sequence, 16 per warp, over its own pages, causal. These are few next
+// to the shared ones, so mma.sync does; at 40 sequences of up to 190 tokens above it takes 99 us, 5 % of the call, and half of what it
+// moves are the shared pages' results (77 MB).
 // grid: (row tiles, G, B); 128 threads.
 template <int HD> struct OwnRows {
     static constexpr int STAGE = 2 * PAGE * HD * 2, STAGES = 2, SMEM = STAGES * STAGE + 1024;
@@ -886,7 +921,7 @@ extern "C" int lp_attention_shared(const void* q, void* out, const void* pages, 
     if (B > 65535 || G > 65535 || num_pages * 2 * G * PAGE > 0x7fffffffll || ((uintptr_t)q | (uintptr_t)pages | (uintptr_t)out) & 15)
         LP_REFUSE("attention_shared: %d sequences, %lld pages for %d heads, or operands that are not aligned to 16 bytes", B, num_pages, G);
     const int R = H / G, one_tile = T <= ROWS / R;
-    SharedArgs s = {table, q_start, kv_len, part_o, part_ml, B, T, H, G, R, shared_pages, splits > 0 ? splits : 1, scale * LOG2E, status};
+    SharedArgs s = {(const __nv_bfloat16*)pages, num_pages, table, q_start, kv_len, part_o, part_ml, B, T, H, G, R, shared_pages, splits > 0 ? splits : 1, scale * LOG2E, status};
     OwnArgs o = {(const __nv_bfloat16*)q, (__nv_bfloat16*)out, table, width, q_start, kv_len, part_o, part_ml, B, T, H, G, R, shared_pages,
                  one_tile ? 2 * splits : splits, splits == 0, scale * LOG2E, status};
     return hd == 64 ? run<64>(q, pages, num_pages, max_new, s, o, stream) : run<128>(q, pages, num_pages, max_new, s, o, stream);

@@ -10,16 +10,18 @@ namespace {
 // and own pages begin are sums over the sequences before it; every CTA forms those it needs itself (a few thousand integers at most,
 // from L2), so one launch does and nothing has to be zero before it. Bound by latency: 3 us for 8 sequences, 4.3 us for 250 sequences of
 // up to 130 tokens on 500 shared pages (B200; 0.67 MB, 0.1 us of memory time). A long sequence is shared by the CTAs along y.
-__device__ __forceinline__ int blocks_of(int length, int page_size) { return length > 0 ? (length + page_size - 1) / page_size : 0; }
+__device__ __forceinline__ int blocks_of(int length, int page_size) { return length > 0 ? (length - 1) / page_size + 1 : 0; }
+// Lengths that no cache has wrap around: what lies outside a tensor is left out by its unsigned index.
+__device__ __forceinline__ int plus(int a, int b) { return (int)((unsigned)a + (unsigned)b); }
 
 __device__ __forceinline__ int block_sum_int(int v, int* scratch) {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    for (int o = 16; o > 0; o >>= 1) v = plus(v, __shfl_xor_sync(0xffffffffu, v, o));
     __syncthreads();
     if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = v;
     __syncthreads();
     int total = 0;
-    for (int w = 0; w < (blockDim.x >> 5); ++w) total += scratch[w];
+    for (int w = 0; w < (blockDim.x >> 5); ++w) total = plus(total, scratch[w]);
     return total;
 }
 
@@ -33,29 +35,30 @@ step_tables_kernel(const int* __restrict__ first, const int* __restrict__ count,
     const int b = blockIdx.x;
     int before = 0, own_before = 0;
     for (int i = threadIdx.x; i < b; i += blockDim.x) {
-        before += max(count[i], 0);
-        own_before += max(0, blocks_of(first[i] + count[i], page_size) - num_shared);
+        const int more = max(count[i], 0);
+        before = plus(before, more);
+        own_before = plus(own_before, max(0, blocks_of(plus(first[i], more), page_size) - num_shared));
     }
     before = block_sum_int(before, scratch);
     own_before = block_sum_int(own_before, scratch);
-    const int from = first[b], n = max(count[b], 0), length = from + n, blocks = blocks_of(length, page_size);
+    const int from = first[b], n = max(count[b], 0), length = plus(from, n), blocks = blocks_of(length, page_size);
     const int step = gridDim.y * blockDim.x, i0 = blockIdx.y * blockDim.x + threadIdx.x;
     if (q_start && i0 == 0) {
         q_start[b] = before;
         kv_len[b] = length;
-        if (b == B - 1) q_start[B] = before + n;
+        if (b == B - 1) q_start[B] = plus(before, n);
     }
     if (positions)
-        for (int i = i0; i < n; i += step)
-            if (before + i < tokens) {
-                positions[before + i] = from + i;
-                seq_ids[before + i] = b;
+        for (int i = i0; i < min(n, tokens); i += step)
+            if ((unsigned)plus(before, i) < (unsigned)tokens) {
+                positions[plus(before, i)] = plus(from, i);
+                seq_ids[plus(before, i)] = b;
             }
     for (int i = i0; i < width; i += step) {
         int page = 0;
         if (i < blocks) {
-            const int at = own_before + i - num_shared;
-            page = i < num_shared ? shared[i] : (at < num_own ? own[at] : 0);
+            const int at = plus(own_before, i - num_shared);
+            page = i < num_shared ? shared[i] : ((unsigned)at < (unsigned)num_own ? own[at] : 0);
         }
         table[(long long)b * width + i] = page;
     }
@@ -103,7 +106,10 @@ int launch_copies(void* storage, int runs, long long run_stride, int vectors, co
 // q_start [B + 1], kv_len [B], positions and seq_ids [tokens].
 extern "C" int lp_step_tables(const int* first, const int* count, const int* shared, int num_shared, const int* own, int num_own, int* q_start,
                               int* kv_len, int* positions, int* seq_ids, int tokens, int* table, int width, int B, int page_size, cudaStream_t stream) {
-    if (B <= 0 || width <= 0 || num_shared < 0 || num_own < 0 || tokens < 0 || page_size <= 0) LP_REFUSE("step_tables: %d sequences, tables of %d pages", B, width);
+    // indexes run past an end by a step of the grid at most
+    const int most = 0x7fffffff - 64 * 256;
+    if (B <= 0 || width <= 0 || width > most || num_shared < 0 || num_own < 0 || tokens < 0 || tokens > most || page_size <= 0)
+        LP_REFUSE("step_tables: %d sequences, tables of %d pages, %d tokens", B, width, tokens);
     // four entries per thread or more
     const long long per_sequence = (tokens > (long long)B * width ? tokens / B : width) / 1024;
     const unsigned shares = (unsigned)(per_sequence < 1 ? 1 : per_sequence > 64 ? 64 : per_sequence);

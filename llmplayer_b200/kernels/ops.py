@@ -1318,8 +1318,10 @@ def attention_shared(q: torch.Tensor, out: torch.Tensor, pages: torch.Tensor, pa
 
     ``q``, ``out``: bfloat16 [T, H * hd], the new tokens of the sequences one behind the other; ``q_start`` int32 [B + 1]: where
     each sequence's begin (a sequence may have none); ``kv_len`` int32 [B]: lengths with the new tokens; ``max_new``: no sequence has
-    more new tokens. A token sees its sequence's keys up to its own position. What rows of ``q`` behind the last sequence hold does not
-    matter, and those of ``out`` stay as they are. ``scratch(name, shape, dtype)`` supplies buffers for partial results."""
+    more new tokens. A token sees its sequence's keys up to its own position; positions that no
+    sequence has reached may hold anything. What rows of ``q`` behind the last sequence hold does not
+    matter, and those of ``out`` stay as they are. ``scratch(name, shape, dtype)`` supplies the buffer of the partial results; calls
+    that may run at the same time (on two streams, or a graph's replay beside a call) need one each."""
     what = "attention_shared"
     _check_attention(q, out, pages, page_table, num_heads, num_kv_heads, head_dim, what)
     _want_all(what, "q_start kv_len", torch.int32, 1, q_start, kv_len)

@@ -75,6 +75,26 @@ def test_tables_stay_within_their_tensors():
 
 
 @pytest.mark.gpu
+def test_tables_of_lengths_that_no_cache_has():
+    """Counts below zero count as none; sums that wrap around write nothing outside the tensors and end."""
+    most = 2 ** 31 - 1
+    for first, count in (([70, 5, 130], [-90, 3, 70]), ([most, most, 3], [1, 1, 2]), ([0, 7, 64], [most, most, 5]), ([-most, -1, 0], [most, 2, most])):
+        room = torch.full((200,), -7, **INT)
+        q_start, kv_len, positions, seq_ids, table = room[4:8], room[12:15], room[20:60], room[64:104], room[120:150].view(3, 10)
+        keep = torch.ones(room.numel(), dtype=torch.bool)
+        for a, b in ((4, 8), (12, 15), (20, 60), (64, 104), (120, 150)):
+            keep[a:b] = False
+        own = torch.arange(1000, 1012, **INT)
+        ops.step_tables(torch.tensor(first, **INT), torch.tensor(count, **INT), torch.tensor([3], **INT), own, q_start, kv_len, positions, seq_ids, table)
+        torch.cuda.synchronize()
+        assert (room.cpu()[keep] == -7).all()
+        assert bool(((table == 0) | (table == 3) | ((table >= 1000) & (table < 1012))).all())
+        if min(count) == -90:
+            assert q_start.tolist() == [0, 0, 3, 73] and kv_len.tolist() == [70, 8, 200]
+            assert table[:, :5].tolist() == [[3, 1000, 0, 0, 0], [3, 0, 0, 0, 0], [3, 1001, 1002, 1003, 0]]
+
+
+@pytest.mark.gpu
 def test_tables_refusals():
     def ints(*v):
         return torch.tensor(v, **INT)
@@ -248,6 +268,20 @@ def test_empty_sequences_and_rows_behind_the_last(H, G, hd):
                          ([0, 0, 1], [0, 0, start + 2]), ([1, 1], [start, start - 63]), ([70, 3, 1], [start + 2, 3, 100]), ([0], [start + 7])):
         case = batch(shared, lengths, new, H, G, hd, seed=len(new), extra_rows=37)
         check(case, shared, H, G, hd, "shared prefix, gaps", f"new {new}, lengths {lengths}")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("H,G,hd", [(8, 2, 64), (32, 8, 128)])
+@pytest.mark.parametrize("junk", [float("nan"), float("inf")])
+def test_shared_pages_that_are_not_full(H, G, hd, junk):
+    """Every sequence ends inside the shared pages: what lies there behind the longest is not looked at."""
+    for shared, lengths, new in ((1, [5, 3], [1, 1]), (3, [130, 129, 2], [1, 1, 1]), (5, [200, 64, 199], [3, 60, 199]), (9, [64] * 3, [1] * 3), (40, [1000] * 70, [1] * 70),
+                                 (21, [900 + i for i in range(12)], [2 + 9 * i for i in range(12)]), (30, [1280, 0], [1, 0]), (1, [64, 64], [64, 1])):
+        case = batch(shared, lengths, new, H, G, hd, seed=shared)
+        pages, table, reached = case[1], case[2], max(lengths)
+        for i in range(shared):
+            pages[table[0, i].long(), :, :, max(0, min(PAGE, reached - i * PAGE)):] = junk
+        check(case, shared, H, G, hd, "shared prefix, short sequences", f"{shared} pages, lengths up to {reached}, {H} on {G} of {hd}")
 
 
 @pytest.mark.gpu
