@@ -159,7 +159,7 @@ class Engine:
             width = 8
             while width < longest + 1:
                 width *= 2
-        elif (self.runtime.device.type == "cuda"
+        elif (tables and self.runtime.device.type == "cuda"
               and 2 * len(tokens) + sum(len(t) for group in tables for t in group) >= StepContext.ON_DEVICE_ENTRIES):
             return StepContext(self.workspace, sequences, tokens, tables, rows, shared_pages=shared, on_device=True)
         return StepContext(self.workspace, sequences, tokens, tables, rows, min_table_width=width, shared_pages=shared)

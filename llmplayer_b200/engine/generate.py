@@ -21,6 +21,7 @@ import time
 from dataclasses import dataclass, field
 from typing import Callable, List, Optional, Sequence
 
+from ..kernels.ops import TOP_LOGPROBS_MOST
 from ..sampling.params import SamplerConfig
 from ..sampling.sampler import SequenceSampler
 
@@ -127,6 +128,9 @@ class GenerationLoop:
                 responses[i] = GenerationResponse(
                     [], n, "error",
                     error=f"Error: prompt too long ({n} tokens, max {self.context_length - 1})")
+            elif req.logprobs is not None and not 0 <= req.logprobs <= TOP_LOGPROBS_MOST:
+                responses[i] = GenerationResponse(
+                    [], n, "error", error=f"Error: the {req.logprobs} most likely tokens cannot be listed (at most {TOP_LOGPROBS_MOST})")
             elif req.max_tokens <= 0:
                 responses[i] = GenerationResponse([], n, "length")
             elif not one_prompt and not self.backend.fits([self._need(req)]):

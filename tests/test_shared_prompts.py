@@ -10,6 +10,7 @@ import dopuvik_helpers
 import helpers
 import plain_llama as P
 import ramupel_helpers
+import vomotar_helpers
 from helpers import check_error, make_model, plain_logits, random_tokens, relative_error, tolerance
 from llmplayer_b200.cache.pages import PAGE_SIZE, PageMap
 from llmplayer_b200.cache.sequence_cache import KVRequest, RowsRequest, SequenceCache, StateRequest
@@ -199,6 +200,15 @@ def test_the_loop_runs_one_prompt_once():
     assert sorted(be.free) == list(range(20))
 
 
+@pytest.mark.parametrize("logprobs", [-1, 33])
+def test_lists_of_a_length_that_is_not_offered_are_refused(logprobs):
+    be = ScriptedBackend()
+    loop = GenerationLoop(be, max_batch=4, context_length=64)
+    out = loop.run([GenerationRequest([1, 2], max_tokens=3, logprobs=logprobs), GenerationRequest([3], max_tokens=2, logprobs=1)])
+    assert out[0].finish_reason == "error" and "most likely" in out[0].error and out[0].token_ids == []
+    assert len(out[1].logprobs) == 2
+
+
 def test_command_line_options():
     o = CLIOptions.parse(["x", "--samples", "5", "--logprobs", "3"])
     assert o.samples == 5 and o.logprobs == 3
@@ -292,6 +302,27 @@ def test_forks_of_designs_with_states_and_windows(tmp_path, monkeypatch, kit, na
             check_error("forks against their parent, float32", f"{kit.__name__} {name}", relative_error(row, ref[0]), 2e-5)
     for s in [parent] + forks:
         eng.release(s)
+    eng.check()
+
+
+@pytest.mark.gpu
+def test_long_steps_of_a_design_without_pages(tmp_path):
+    """Nothing is cached but states: there is no table that a long step could describe on the device."""
+    from llmplayer_b200 import Engine
+    from llmplayer_b200.engine.step import StepContext
+    eng = Engine.load(vomotar_helpers.make_model(tmp_path, "recurrent", "float32"), dtype="float32", max_tokens=4096, max_slots=4)
+    assert eng.cache.groups == []
+    prompt = random_tokens(StepContext.ON_DEVICE_ENTRIES + 76, eng.vocab_size, seed=8)
+    slot, other = eng.acquire(), eng.acquire()
+    got = eng.step([(slot, prompt)], [[len(prompt) - 1]]).cpu()
+    for a in range(0, len(prompt), 100):
+        want = eng.step([(other, prompt[a:a + 100])], [[99]]).cpu()
+    # float32 sums over chunks of other lengths: two factors of 1100 terms' rounding, 2 * 1100 * 2^-24
+    check_error("a long step without pages", "float32", relative_error(got[0], want[0]), 1.4e-4)
+    for fork in eng.fork(slot, 2):
+        eng.release(fork)
+    eng.release(slot)
+    eng.release(other)
     eng.check()
 
 
