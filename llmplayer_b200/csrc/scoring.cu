@@ -14,6 +14,10 @@
 // warp keeps its k first tokens sorted over its lanes, and a logit is looked at again only if it is not below a bound that the
 // warps' largest logits so far give. A cluster of CTAs shares a long row when the rows are few; their parts meet in the first CTA's
 // registers through distributed shared memory, so there is no scratch in memory and no order of arrival: results repeat bit for bit.
+//
+// Bound by memory at many rows: 2,000 rows of 128,256 float32 logits (1.03 GB, 157 us at the measured copy rate) take 180 us without
+// a list, 87 %, 193 to 209 with the 2 and 260 with the 20 most likely tokens (B200, caches cold): a row's first load fills the lists of its
+// eight warps, and a logit costs about four issue slots. At few rows bound by latency: 16 us for one row of 128,256 and for 8, with 5 tokens.
 #include "common.cuh"
 
 #include <type_traits>
@@ -328,9 +332,10 @@ token_logprobs_kernel(const T* __restrict__ logits, long long ld, const int* __r
         if (TOP) {
             lane_most = fmaxf(lane_most, most);
             if ((turn & (turn + 1)) == 0 && (turn == 0 || to - w0 > turn * PER * THREADS)) {
-                // At first, and whenever as much has been seen again as before and most is still to come: of the lanes' largest logits so far the k-th largest has k logits that are not below it. And each warp posts a key that
-                // per_warp of its lanes are not below: what is not above enough warps' keys is not above k logits. Posts only rise, so an
-                // old one holds as well. (-inf may stand for no logit at all.)
+                // At first, and whenever as much has been seen again as before and most is still to come: of the lanes' largest logits so
+                // far the k-th largest has k logits that are not below it. And each warp posts a key that per_warp of its lanes are not
+                // below: what is not above enough warps' keys is not above k logits. Posts only rise, so an old one holds as well.
+                // (-inf may stand for no logit at all.)
                 const uint32_t key = order_key(lane_most);
                 const uint32_t sorted = sort32(key > 0x007fffffu ? key : 0u, lane), mine = __shfl_sync(ALL, sorted, per_warp - 1);
                 bound = max(bound, __shfl_sync(ALL, sorted, top - 1));
@@ -508,7 +513,9 @@ extern "C" int lp_token_logprobs(const void* logits, int dtype, long long ld, co
                                  int* top_ids, float* top_logprobs, int rows, int V, int top, cudaStream_t stream) {
     if (rows <= 0 || V <= 0 || top < 0 || top > MOST_TOP || top > V || ld < V || rows > 0x7fffffff / MOST_CLUSTER || V > 0x7fffffff - 4 * THREADS * VALUES)
         LP_REFUSE("token_logprobs: %d rows of %d logits, the %d most likely", rows, V, top);
-    // few rows: as many CTAs per row as the GPU holds at once, each with a whole load of its threads at least
+    // Few rows: as many CTAs per row as the GPU holds at once, each with half a load of its threads at least. B200, 128,256 float32 logits,
+    // 5 tokens, us with 1, 2, 4 and 8 CTAs per row: 1 row 35, 25, 21, 16; 48 rows 37, 27, 25, 23; 100 rows 37, 33, 29, 41;
+    // 220 rows 45, 41, 57, 72; 300 rows 55, 59, 68, 92; 8 rows of 2,000 10, 12, 12, 12; 1 row of 32,000 18, 16, 14, 12.
     int cluster = 1;
     while (cluster < MOST_CLUSTER && (long long)rows * cluster * 2 <= (long long)lp_sm_count() * CTAS_PER_SM && V / (cluster * 2) >= THREADS * VALUES / 2) cluster *= 2;
     if (dtype == LP_F32)
