@@ -584,14 +584,14 @@ class Engine:
     def generate_samples(self, prompt: Sequence[int], samples: int, sampler_config=None, *, max_tokens: int = 256,
                          stop_token_ids=None, logprobs: Optional[int] = None):
         """``samples`` continuations of one prompt, drawn side by side: the prompt is run once, its cached pages are shared, and a decode
-        step attends over them once for all. Sample i draws with the configuration's seed plus i. Returns one
-        :class:`GenerationResponse` per sample."""
+        step attends over them once for all. The first sample draws with the configuration's seed, the others with seeds spread from it
+        (:meth:`SamplerConfig.for_sample`). Returns one :class:`GenerationResponse` per sample."""
         from ..sampling.params import SamplerConfig
         from .generate import GenerationLoop, GenerationRequest
         if int(samples) < 1:
             raise RequestError(f"{samples} samples of a prompt")
         config = sampler_config if sampler_config is not None else SamplerConfig()
-        requests = [GenerationRequest(prompt_ids=list(prompt), max_tokens=max_tokens, sampler_config=config.with_seed(config.seed + i),
+        requests = [GenerationRequest(prompt_ids=list(prompt), max_tokens=max_tokens, sampler_config=config.for_sample(i),
                                       stop_token_ids=stop_token_ids, logprobs=logprobs) for i in range(int(samples))]
         total = min(len(requests[0].prompt_ids) + max(0, max_tokens), self.context_length)
         shared = len(requests[0].prompt_ids) // PAGE_SIZE

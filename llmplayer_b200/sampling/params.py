@@ -52,6 +52,17 @@ class SamplerConfig:
     def with_seed(self, seed: int) -> "SamplerConfig":
         return replace(self, seed=seed)
 
+    def for_sample(self, i: int) -> "SamplerConfig":
+        """The options of the i-th of several samples of one prompt: the first draws with the seed itself, the others with seeds spread
+        from it. (Neighbouring seeds will not do: the generator's first draws hardly differ between them. The mixing function is
+        splitmix64's, by Steele, Lea and Flood.)"""
+        if i == 0:
+            return self
+        z = (int(self.seed) + i * 0x9E3779B97F4A7C15) & 0xFFFFFFFFFFFFFFFF
+        z = ((z ^ (z >> 30)) * 0xBF58476D1CE4E5B9) & 0xFFFFFFFFFFFFFFFF
+        z = ((z ^ (z >> 27)) * 0x94D049BB133111EB) & 0xFFFFFFFFFFFFFFFF
+        return replace(self, seed=z ^ (z >> 31))
+
     @property
     def is_greedy(self) -> bool:
         return self.temperature == 0.0

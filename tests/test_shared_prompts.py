@@ -18,6 +18,7 @@ from llmplayer_b200.cli import CLIOptions
 from llmplayer_b200.engine.generate import GenerationLoop, GenerationRequest
 from llmplayer_b200.engine.scoring import TokenLogprob
 from llmplayer_b200.errors import CacheError, CacheFull, RequestError
+from llmplayer_b200.sampling.params import SamplerConfig
 
 
 # ------------------------------------------------------------------------------------------------ bookkeeping, on the CPU
@@ -207,6 +208,16 @@ def test_lists_of_a_length_that_is_not_offered_are_refused(logprobs):
     out = loop.run([GenerationRequest([1, 2], max_tokens=3, logprobs=logprobs), GenerationRequest([3], max_tokens=2, logprobs=1)])
     assert out[0].finish_reason == "error" and "most likely" in out[0].error and out[0].token_ids == []
     assert len(out[1].logprobs) == 2
+
+
+@pytest.mark.parametrize("seed", [0, 5, 2 ** 63 - 1, -3, 1234567890123])
+def test_first_draws_of_samples_are_spread(seed):
+    from llmplayer_b200.sampling.java_random import JavaRandom
+    config = SamplerConfig(seed=seed)
+    assert config.for_sample(0) == config
+    draws = sorted(JavaRandom(config.for_sample(i).seed).next_float() for i in range(400))
+    # 400 independent uniform draws: the largest distance to the even spread exceeds 2.2 / sqrt(400) once in 8,000 times
+    assert max(max((i + 1) / 400 - x, x - i / 400) for i, x in enumerate(draws)) < 0.11
 
 
 def test_command_line_options():
