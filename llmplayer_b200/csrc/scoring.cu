@@ -46,13 +46,13 @@ __device__ __forceinline__ float key_value(uint32_t k) {
 __device__ __forceinline__ uint64_t entry(float x, int i) { return ((uint64_t)order_key(x) << 32) | (uint32_t)~i; }
 __device__ __forceinline__ bool before(float x, int i, float y, int j) { return entry(x, i) > entry(y, j); }
 
-// 32 keys or entries, one per lane, in falling order
-template <typename K> __device__ __forceinline__ K sort32(K v, int lane) {
+// 32 entries, one per lane, in falling order
+__device__ __forceinline__ uint64_t sort32(uint64_t v, int lane) {
 #pragma unroll
     for (int size = 2; size <= 32; size <<= 1)
 #pragma unroll
         for (int stride = size >> 1; stride > 0; stride >>= 1) {
-            const K w = __shfl_xor_sync(ALL, v, stride);
+            const uint64_t w = __shfl_xor_sync(ALL, v, stride);
             const bool larger = ((lane & stride) == 0) == ((lane & size) == 0);
             v = (v > w) == larger ? v : w;
         }
@@ -122,19 +122,7 @@ struct Sums {
         c = 0.f;
         m = to;
     }
-    __device__ __forceinline__ void add(Sums o) {
-        if (o.m > m) lower(o.m);
-        else if (o.m < m) o.lower(m);
-        c += o.c;
-        r += o.r;
-        u += o.u;
-        ahead += o.ahead;
-    }
 };
-__device__ __forceinline__ Sums shuffled(const Sums& s, int o) {
-    return {__shfl_xor_sync(ALL, s.m, o), __shfl_xor_sync(ALL, s.c, o), __shfl_xor_sync(ALL, s.r, o), __shfl_xor_sync(ALL, s.u, o),
-            __shfl_xor_sync(ALL, s.ahead, o)};
-}
 
 // ------------------------------------------------------------------ loads: 16 bytes at a time, the row's ends one by one
 template <typename T> struct Vec;
@@ -257,8 +245,32 @@ token_logprobs_kernel(const T* __restrict__ logits, long long ld, const int* __r
         __syncwarp();
     };
     const int per_warp = (top + WARPS - 1) / WARPS, warps_needed = per_warp ? (top + per_warp - 1) / per_warp : 0;
+    float lane_most = -INFINITY;
     uint32_t bound = 0;                  // no logit below this key is among the first k
-    float cut = key_value(0), lane_most = -INFINITY;
+    // Each warp posts a key that per_warp of its lanes have a logit at or above: enough warps' keys are below k logits or are them.
+    // (-inf may stand for no logit at all.)
+    auto warps_key = [&]() {
+        uint32_t key = order_key(lane_most), most = 0;
+        if (key <= 0x007fffffu) key = 0;
+        for (int i = 0; i < per_warp; ++i) {
+            most = __reduce_max_sync(ALL, key);
+            if (lane == __ffs(__ballot_sync(ALL, key == most)) - 1) key = 0;
+        }
+        return most;
+    };
+    auto posts_bound = [&]() {
+        const volatile uint32_t* const posted = posts;
+        const uint32_t post = lane < WARPS ? posted[lane] : 0u;
+        int place = 0;
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) {
+            const uint32_t other = __shfl_sync(ALL, post, w);
+            if (other > post || (other == post && w < lane)) ++place;
+        }
+        const uint32_t who = __ballot_sync(ALL, lane < WARPS && place == warps_needed - 1);
+        return __shfl_sync(ALL, post, __ffs(who) - 1);
+    };
+    float cut = key_value(0);
     int turn = 0;
     for (int w0 = from; w0 < to; w0 += PER * THREADS) {
         float v[VALUES];
@@ -332,25 +344,13 @@ token_logprobs_kernel(const T* __restrict__ logits, long long ld, const int* __r
         if (TOP) {
             lane_most = fmaxf(lane_most, most);
             if ((turn & (turn + 1)) == 0 && (turn == 0 || to - w0 > turn * PER * THREADS)) {
-                // At first, and whenever as much has been seen again as before and most is still to come: of the lanes' largest logits so
-                // far the k-th largest has k logits that are not below it. And each warp posts a key that per_warp of its lanes are not
-                // below: what is not above enough warps' keys is not above k logits. Posts only rise, so an old one holds as well.
-                // (-inf may stand for no logit at all.)
-                const uint32_t key = order_key(lane_most);
-                const uint32_t sorted = sort32(key > 0x007fffffu ? key : 0u, lane), mine = __shfl_sync(ALL, sorted, per_warp - 1);
-                bound = max(bound, __shfl_sync(ALL, sorted, top - 1));
+                // At first, and whenever as much has been seen again as before and most is still to come. Posts only rise, so an old one
+                // holds as well.
+                const uint32_t key = warps_key();
                 volatile uint32_t* const posted = posts;
-                if (lane == 0) posted[warp] = mine;
+                if (lane == 0) posted[warp] = key;
                 if (turn == 0) __syncthreads();
-                const uint32_t post = lane < WARPS ? posted[lane] : 0u;
-                int place = 0;
-#pragma unroll
-                for (int w = 0; w < WARPS; ++w) {
-                    const uint32_t other = __shfl_sync(ALL, post, w);
-                    if (other > post || (other == post && w < lane)) ++place;
-                }
-                const uint32_t who = __ballot_sync(ALL, lane < WARPS && place == warps_needed - 1);
-                bound = max(bound, __shfl_sync(ALL, post, __ffs(who) - 1));
+                bound = max(bound, posts_bound());
                 cut = key_value(max(bound, (uint32_t)(kth >> 32)));
             }
             ++turn;
@@ -388,15 +388,35 @@ token_logprobs_kernel(const T* __restrict__ logits, long long ld, const int* __r
     lp_grid_release();
 
     // ---------------------------------------------------------------- the warps' parts, then the CTAs'
+    // a warp's lanes have one maximum
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) s.add(shuffled(s, o));
+    for (int o = 16; o > 0; o >>= 1) {
+        s.c += __shfl_xor_sync(ALL, s.c, o);
+        s.r += __shfl_xor_sync(ALL, s.r, o);
+        s.u += __shfl_xor_sync(ALL, s.u, o);
+    }
+    s.ahead = __reduce_add_sync(ALL, s.ahead);
     if (lane == 0) parts[warp] = s;
-    if (TOP && threadIdx.x == 0) found.count = 0;
+    if (TOP) {
+        const uint32_t key = warps_key();
+        if (lane == 0) posts[warp] = key;
+        if (threadIdx.x == 0) found.count = 0;
+    }
     __syncthreads();
     const Sums nothing = {-INFINITY, 0.f, 0.f, 0.f, 0};
-    auto sums_meet = [&]() {                                     // those of a warp's lanes, in all of them
+    static_assert(WARPS <= 8 && MOST_CLUSTER <= 8, "parts meet in eight lanes");
+    auto sums_meet = [&]() {                                     // those of a warp's first eight lanes
+        float most = s.m;
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) s.add(shuffled(s, o));
+        for (int o = 4; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(ALL, most, o));
+        if (s.m < most) s.lower(most);
+#pragma unroll
+        for (int o = 4; o > 0; o >>= 1) {
+            s.c += __shfl_xor_sync(ALL, s.c, o);
+            s.r += __shfl_xor_sync(ALL, s.r, o);
+            s.u += __shfl_xor_sync(ALL, s.u, o);
+            s.ahead += __shfl_xor_sync(ALL, s.ahead, o);
+        }
     };
     if (warp == 0) {
         s = lane < WARPS ? parts[lane] : nothing;
@@ -415,14 +435,15 @@ token_logprobs_kernel(const T* __restrict__ logits, long long ld, const int* __r
     };
     int candidates = 0;
     if (TOP) {
-        const uint32_t listed = __ballot_sync(ALL, list != 0 && lane < top);
+        bound = max(bound, posts_bound());
+        const uint64_t other = lane < held ? pending[warp][lane] : 0;        // fewer than 32
+        const bool a = lane < top && list != 0 && (uint32_t)(list >> 32) >= bound, b = other != 0 && (uint32_t)(other >> 32) >= bound;
+        const uint32_t listed = __ballot_sync(ALL, a), others = __ballot_sync(ALL, b), before_me = (1u << lane) - 1;
         int at = 0;
-        if (lane == 0) at = atomicAdd(&found.count, __popc(listed) + held);
+        if (lane == 0) at = atomicAdd(&found.count, __popc(listed) + __popc(others));
         at = __shfl_sync(ALL, at, 0);
-        if (list != 0 && lane < top) found.pool[at + lane] = list;
-        at += __popc(listed);
-        __syncwarp();
-        for (int i = lane; i < held; i += 32) found.pool[at + i] = pending[warp][i];
+        if (a) found.pool[at + __popc(listed & before_me)] = list;
+        if (b) found.pool[at + __popc(listed) + __popc(others & before_me)] = other;
         if (warp == 0) found.best[lane] = 0;
         __syncthreads();
         candidates = found.count;
