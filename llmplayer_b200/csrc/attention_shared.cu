@@ -14,9 +14,9 @@
 // B200, 32 query heads on 8, caches cold, the whole call in a graph, against attention that reads every sequence's pages:
 //   64 single tokens, heads of 128, 128 shared pages, up to 250 own positions each: 39 us against 432; the two kernels by
 //       themselves 21 and 15 us for 70 MB (10.8 us at the measured copy rate).
-//   24 sequences of 9 to 37 tokens, heads of 64, 50 shared pages: 45 against 234; 34 and 13 us for 15 GFLOP.
-//   40 sequences of 47 to 190 tokens, heads of 128, 500 shared pages: 2,090 against 5,390; 2,050 and 99 us, 1,175 TFLOP/s, 72 % of
-//       the measured rate of dense products; 2,370 over a long run, where the power limit holds the clock down.
+//   24 sequences of 9 to 37 tokens, heads of 64, 50 shared pages: 43 against 234; 32 and 13 us for 15 GFLOP.
+//   40 sequences of 47 to 190 tokens, heads of 128, 500 shared pages: 1,890 against 5,390, 1,298 TFLOP/s, 80 % of the measured rate of
+//       dense products (99 us of it the second kernel); 2,100 over a long run, where the power limit holds the clock down.
 //
 // All sums, maxima and partial results are float32. The softmax weights enter the products with the values as bfloat16, rounded
 // against a reference maximum (as in the other attention kernels here); the row sums use the float32 weights.
@@ -39,11 +39,12 @@ constexpr float RESCALE_ABOVE = 8.0f;     // log2: how far a row's reference max
 //   ->  O[128 x HD] += P V (P from tensor memory, V from shared memory, contiguous in N).
 // A chain has two S tiles: the scores of its next page are asked for before it has finished with one. (With one tile of 128 keys
 // per chain the two chains' softmaxes ran one behind the other: 4,000 cycles per 128 keys at heads of 128.)
-// What bounds it: a page of 64 keys takes 1,700 to 2,000 cycles for both chains. The products alone take 1,650 of them (two of
-// 128 x 64 x 128 each way), the softmaxes alone 1,760 (1,024 of those are the exp2 unit's: 2 x 128 x 64 at 16 per cycle). At the 500
-// pages above these took longer than the 2,020 to 2,090 us: a fixed order between the chains 2,386, two groups of softmax warps per chain
-// 2,061, blocks of 128 keys on two threads per row 2,526, weights in tiles of their own and scores given back early 2,150; a polynomial
-// for part of the exponentials gave less than 2 %.
+// What bounds it: a page of 64 keys takes both chains 1,550 to 1,600 cycles. The products alone take 1,650 back to back at heads of 128 (half of
+// that at 64); a chain's page has 600 cycles of exponentials (64 per thread, 8 cycles per warp: the exp2 unit's rate) and 600 of waiting,
+// loading, the maximum and the store. At the 500 pages above these took longer than the 1,870 to 1,900 us: chains that take no turns 2,060 (and 529
+// against 472 at heads of 64, 300 pages), turns of whole chains 2,386, two groups of softmax warps per chain 2,061, blocks of 128 keys on
+// two threads per row 2,526, weights in tiles of their own and scores given back early 2,150. A polynomial for a quarter of the
+// exponentials gained 5 % at heads of 64 without turns, and lost with them.
 template <int HD> struct Shape {
     static constexpr int BLOCKS = HD / 64;                          // blocks of 64 features (one swizzle row each)
     static constexpr int TILE = PAGE * HD * 2;                      // keys or values of a page
@@ -323,10 +324,23 @@ attention_shared_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
         const int count = turns(c);
         float m = NEG_BIG, l = 0.f;
         bool ok = true;
+        // The two chains' warps of a scheduler take turns at the exponentials (named barriers of 64): while one has the exp2 unit the other loads,
+        // looks for its maximum and stores. Left to themselves both come to their exponentials together and then leave the unit idle together.
+        const bool take_turns = !alone && chains == 2;
+        const int mine = 2 + quarter * 2 + c, theirs = 2 + quarter * 2 + (c ^ 1);
+        auto await_turn = [&]() { if (take_turns) asm volatile("bar.sync %0, 64;" ::"r"(mine) : "memory"); };
+        auto hand_on = [&](int k) { if (take_turns && (c == 0 || k + 1 < count)) asm volatile("bar.arrive %0, 64;" ::"r"(theirs) : "memory"); };
+        auto give_up = [&](int k) {                                // at page k: the other chain goes on, without an end to its waits otherwise
+            for (; take_turns && k < count; ++k) {
+                await_turn();
+                hand_on(k);
+            }
+        };
+        if (c == 1) hand_on(-1);
         for (int k = 0; k < count; ++k) {
             const uint32_t s_addr = lane_addr + SH::S_COL + c * 128 + (k & 1) * PAGE;
             ok = __all_sync(0xffffffffu, mbar_wait(&s_ready[c * 2 + (k & 1)], (k >> 1) & 1));
-            if (!ok) { if (lane == 0) atomicExch(a.status, 85); break; }
+            if (!ok) { if (lane == 0) atomicExch(a.status, 85); give_up(k); break; }
             tcgen05_fence_after();
             uint32_t s[PAGE];
             tmem_ld32(s_addr, s);
@@ -347,25 +361,28 @@ attention_shared_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
             // The reference follows only when the row's maximum has outgrown it by more than RESCALE_ABOVE; then the output so far comes
             // down to it, which must have been added up before and waits for nothing else (the next product follows p_ready).
             const bool moves = mx > m + RESCALE_ABOVE;
-            if (__any_sync(0xffffffffu, moves) && k > 0) {
-                ok = __all_sync(0xffffffffu, mbar_wait(&o_ready[c], (k - 1) & 1));
-                if (!ok) { if (lane == 0) atomicExch(a.status, 86); break; }
-                tcgen05_fence_after();
-                const float factor = moves ? fast_exp2(m - mx) : 1.0f;
+            if (__any_sync(0xffffffffu, moves)) {
+                if (k > 0) {
+                    ok = __all_sync(0xffffffffu, mbar_wait(&o_ready[c], (k - 1) & 1));
+                    if (!ok) { if (lane == 0) atomicExch(a.status, 86); give_up(k); break; }
+                    tcgen05_fence_after();
+                    const float factor = moves ? fast_exp2(m - mx) : 1.0f;
 #pragma unroll
-                for (int d = 0; d < HD; d += 32) {
-                    uint32_t o[32];
-                    tmem_ld32(o_addr + d, o);
-                    tmem_ld_wait();
+                    for (int d = 0; d < HD; d += 32) {
+                        uint32_t o[32];
+                        tmem_ld32(o_addr + d, o);
+                        tmem_ld_wait();
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * factor);
-                    tmem_st32(o_addr + d, o);
+                        for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * factor);
+                        tmem_st32(o_addr + d, o);
+                    }
+                }
+                if (moves) {
+                    l *= fast_exp2(m - mx);
+                    m = mx;
                 }
             }
-            if (moves) {
-                l *= fast_exp2(m - mx);
-                m = mx;
-            }
+            await_turn();
             float sum4[4] = {0.f, 0.f, 0.f, 0.f};
             uint32_t p[PAGE / 2];
 #pragma unroll
@@ -378,6 +395,7 @@ attention_shared_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
                 p[j] = pack_bf16(e0, e1);
             }
             tmem_st32(s_addr, p);
+            hand_on(k);
             tmem_st_wait();
             l += (sum4[0] + sum4[1]) + (sum4[2] + sum4[3]);
             // A parity tells only a phase from the one before it. The scores of page k say that the products up to page k - 2 have been
