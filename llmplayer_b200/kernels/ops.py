@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes
 import functools
+from array import array
 from ctypes import c_float, c_int, c_void_p
 from dataclasses import dataclass
 from typing import Dict, Optional
@@ -439,6 +440,18 @@ def _want_all(what: str, names: str, dtype, ndim: int, *tensors: torch.Tensor) -
     for t, name in zip(tensors, names.split()):
         _want(t, f"{what} {name}", dtype, ndim)
         _on_current_device(what, t)
+
+
+def _fine(dtype, *tensors: torch.Tensor) -> bool:
+    """Whether all are contiguous tensors of the type on the current device: one quick look before the checks that name what is wrong."""
+    device = torch._C._cuda_getDevice()
+    try:
+        for t in tensors:
+            if t.get_device() != device or t.dtype is not dtype or not t.is_contiguous():
+                return False
+    except AttributeError:
+        return False
+    return True
 
 
 # --------------------------------------------------------------------------- embedding
@@ -1323,17 +1336,22 @@ def attention_shared(q: torch.Tensor, out: torch.Tensor, pages: torch.Tensor, pa
     matter, and those of ``out`` stay as they are. ``scratch(name, shape, dtype)`` supplies the buffer of the partial results; calls
     that may run at the same time (on two streams, or a graph's replay beside a call) need one each."""
     what = "attention_shared"
-    _check_attention(q, out, pages, page_table, num_heads, num_kv_heads, head_dim, what)
-    _want_all(what, "q_start kv_len", torch.int32, 1, q_start, kv_len)
-    _on_current_device(what, q, out, pages, page_table)
-    B, T = kv_len.numel(), q.shape[0]
-    if B == 0 or q_start.numel() != B + 1 or page_table.shape[0] != B:
-        raise KernelError(f"{what}: {B} sequences, {q_start.numel()} offsets, table {tuple(page_table.shape)}")
-    if not attention_shared_serves(num_heads, num_kv_heads, head_dim, pages.shape[3]):
-        raise KernelError(f"{what}: {num_heads} heads on {num_kv_heads} of {head_dim} over pages of {pages.shape[3]} are not served "
+    if not (_fine(torch.bfloat16, q, out, pages) and _fine(torch.int32, page_table, q_start, kv_len) and q_start.dim() == kv_len.dim() == 1):
+        _check_attention(q, out, pages, page_table, num_heads, num_kv_heads, head_dim, what)
+        _want_all(what, "q_start kv_len", torch.int32, 1, q_start, kv_len)
+        _on_current_device(what, q, out, pages, page_table)
+    shape, table, cache = q.shape, page_table.shape, pages.shape
+    if (len(shape) != 2 or len(table) != 2 or len(cache) != 5 or shape[1] != num_heads * head_dim or out.shape != shape
+            or cache[1] != 2 or cache[2] != num_kv_heads or cache[4] != head_dim):
+        _check_attention(q, out, pages, page_table, num_heads, num_kv_heads, head_dim, what)
+    B, T = kv_len.numel(), shape[0]
+    if B == 0 or q_start.numel() != B + 1 or table[0] != B:
+        raise KernelError(f"{what}: {B} sequences, {q_start.numel()} offsets, table {tuple(table)}")
+    if not attention_shared_serves(num_heads, num_kv_heads, head_dim, cache[3]):
+        raise KernelError(f"{what}: {num_heads} heads on {num_kv_heads} of {head_dim} over pages of {cache[3]} are not served "
                           f"(heads of 64 or 128, at most 128 per key head, pages of 64)")
-    if not 0 <= int(shared_pages) <= page_table.shape[1]:
-        raise KernelError(f"{what}: {shared_pages} shared pages in tables of {page_table.shape[1]}")
+    if not 0 <= int(shared_pages) <= table[1]:
+        raise KernelError(f"{what}: {shared_pages} shared pages in tables of {table[1]}")
     if int(max_new) < 1:
         raise KernelError(f"{what}: at most {max_new} new tokens per sequence")
     if T == 0:
@@ -1343,7 +1361,7 @@ def attention_shared(q: torch.Tensor, out: torch.Tensor, pages: torch.Tensor, pa
     part_o = _ptr(parts)
     part_ml = part_o + 4 * slots * T * num_heads * head_dim if slots else None
     lib = library("attention_shared")
-    _check(lib, lib.lp_attention_shared(q.data_ptr(), out.data_ptr(), pages.data_ptr(), pages.shape[0], page_table.data_ptr(), page_table.shape[1],
+    _check(lib, lib.lp_attention_shared(q.data_ptr(), out.data_ptr(), pages.data_ptr(), cache[0], page_table.data_ptr(), table[1],
                                         q_start.data_ptr(), kv_len.data_ptr(), B, T, int(max_new), num_heads, num_kv_heads, head_dim, int(shared_pages),
                                         float(scale), splits, part_o, part_ml, kernel_status().data_ptr(), _stream()))
     return out
@@ -1386,12 +1404,13 @@ def step_tables(first: torch.Tensor, count: torch.Tensor, shared: torch.Tensor, 
     if q_start is None or kv_len is None or positions is None or seq_ids is None:
         if any(t is not None for t in rest):
             raise KernelError(f"{what}: q_start, kv_len, positions and seq_ids go together")
-        _want_all(what, "first count shared own", torch.int32, 1, first, count, shared, own)
-        tokens = 0
-    else:
+        rest = ()
+    if not (_fine(torch.int32, first, count, shared, own, page_table, *rest) and page_table.dim() == 2
+            and first.dim() == count.dim() == shared.dim() == own.dim() == 1
+            and (not rest or q_start.dim() == kv_len.dim() == positions.dim() == seq_ids.dim() == 1)):
         _want_all(what, "first count shared own q_start kv_len positions seq_ids", torch.int32, 1, first, count, shared, own, *rest)
-        tokens = positions.numel()
-    _want_all(what, "page_table", torch.int32, 2, page_table)
+        _want_all(what, "page_table", torch.int32, 2, page_table)
+    tokens = positions.numel() if rest else 0
     B, (rows, width) = first.numel(), page_table.shape
     if B == 0 or count.numel() != B or rows != B or width == 0:
         raise KernelError(f"{what}: {B} sequences, {count.numel()} counts, table {tuple(page_table.shape)}")
@@ -1416,7 +1435,7 @@ def copy_pages(storage: torch.Tensor, sources, targets) -> None:
     if not isinstance(storage, torch.Tensor) or storage.dim() < 3:
         raise KernelError(f"{what}: expected a storage tensor [runs, pages, ...]")
     runs, num_pages = storage.shape[:2]
-    if targets and not (0 <= min(sources) and max(sources) < num_pages and 0 <= min(targets) and max(targets) < num_pages):
+    if targets and not 0 <= min(min(sources), min(targets)) <= max(max(sources), max(targets)) < num_pages:
         raise KernelError(f"{what}: pages {sources} to {targets} of {num_pages}")
     distinct = set(targets)
     if len(distinct) != len(targets) or not distinct.isdisjoint(sources):
@@ -1433,8 +1452,8 @@ def copy_pages(storage: torch.Tensor, sources, targets) -> None:
     most = lib.lp_copy_pages_most()
     for a in range(0, len(targets), most):
         n = min(most, len(targets) - a)
-        pairs = (ctypes.c_int * (2 * n))(*sources[a:a + n], *targets[a:a + n])
-        _check(lib, lib.lp_copy_pages(storage.data_ptr(), runs, num_pages, page_bytes, pairs, n, _stream()))
+        pairs = array("i", sources[a:a + n] + targets[a:a + n])
+        _check(lib, lib.lp_copy_pages(storage.data_ptr(), runs, num_pages, page_bytes, pairs.buffer_info()[0], n, _stream()))
 
 
 # --------------------------------------------------------------------------- latent attention
@@ -2737,28 +2756,33 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, logprob: torch.T
     what = "token_logprobs"
     if not isinstance(logits, torch.Tensor) or not logits.is_cuda:
         raise KernelError(f"{what} logits: expected a CUDA tensor")
-    if logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1) or (logits.shape[0] > 1 and logits.stride(0) < logits.shape[1]):
-        raise KernelError(f"{what} logits: expected rows of consecutive values, got shape {tuple(logits.shape)}, strides {logits.stride()}")
-    code = _code(logits, f"{what} logits")
-    R, V = logits.shape
+    shape, strides = logits.shape, logits.stride()
+    if len(shape) != 2 or (shape[1] > 1 and strides[1] != 1) or (shape[0] > 1 and strides[0] < shape[1]):
+        raise KernelError(f"{what} logits: expected rows of consecutive values, got shape {tuple(shape)}, strides {strides}")
+    R, V = shape
+    code = _CODES.get(logits.dtype)
+    if code is None:
+        code = _code(logits, f"{what} logits")
     _on_current_device(what, logits)
-    _want_all(what, "targets rank", torch.int32, 1, targets, rank)
-    _want_all(what, "logprob entropy", torch.float32, 1, logprob, entropy)
+    if not (_fine(torch.int32, targets, rank) and _fine(torch.float32, logprob, entropy)
+            and targets.dim() == rank.dim() == logprob.dim() == entropy.dim() == 1):
+        _want_all(what, "targets rank", torch.int32, 1, targets, rank)
+        _want_all(what, "logprob entropy", torch.float32, 1, logprob, entropy)
     top = 0
-    if (top_ids is None) != (top_logprobs is None):
-        raise KernelError(f"{what}: top_ids and top_logprobs go together")
-    if top_ids is not None:
+    if top_ids is not None or top_logprobs is not None:
+        if top_ids is None or top_logprobs is None:
+            raise KernelError(f"{what}: top_ids and top_logprobs go together")
         _want_all(what, "top_ids", torch.int32, 2, top_ids)
         _want_all(what, "top_logprobs", torch.float32, 2, top_logprobs)
         top = top_ids.shape[1]
         if top_ids.shape != (R, top) or top_logprobs.shape != (R, top):
             raise KernelError(f"{what}: top_ids {tuple(top_ids.shape)}, top_logprobs {tuple(top_logprobs.shape)} for {R} rows")
-    if targets.numel() != R or logprob.numel() != R or entropy.numel() != R or rank.numel() != R:
+    if not targets.numel() == logprob.numel() == entropy.numel() == rank.numel() == R:
         raise KernelError(f"{what}: {R} rows, {targets.numel()} targets, outputs of {logprob.numel()}, {entropy.numel()}, {rank.numel()}")
     if V == 0 or top > min(V, TOP_LOGPROBS_MOST):
         raise KernelError(f"{what}: the {top} most likely of {V} tokens (at most {TOP_LOGPROBS_MOST})")
     if R == 0:
         return
     lib = library("scoring")
-    _check(lib, lib.lp_token_logprobs(logits.data_ptr(), code, logits.stride(0) if R > 1 else V, targets.data_ptr(), logprob.data_ptr(),
+    _check(lib, lib.lp_token_logprobs(logits.data_ptr(), code, strides[0] if R > 1 else V, targets.data_ptr(), logprob.data_ptr(),
                                       entropy.data_ptr(), rank.data_ptr(), _ptr(top_ids), _ptr(top_logprobs), R, V, top, _stream()))
