@@ -15,9 +15,10 @@
 // warps' largest logits so far give. A cluster of CTAs shares a long row when the rows are few; their parts meet in the first CTA's
 // registers through distributed shared memory, so there is no scratch in memory and no order of arrival: results repeat bit for bit.
 //
-// Bound by memory at many rows: 2,000 rows of 128,256 float32 logits (1.03 GB, 157 us at the measured copy rate) take 180 us without
-// a list, 87 %, 193 to 209 with the 2 and 260 with the 20 most likely tokens (B200, caches cold): a row's first load fills the lists of its
-// eight warps, and a logit costs about four issue slots. At few rows bound by latency: 16 us for one row of 128,256 and for 8, with 5 tokens.
+// Bound by memory at many rows: 2,000 rows of 128,256 float32 logits (1.03 GB, 157 us at the measured copy rate) take 172 us without
+// a list, 91 %, 184 with the 2 and 197 with the 20 most likely tokens (B200, caches cold): a row's first loads fill the lists of its eight
+// warps. At few rows bound by latency: 14 us for one row of 128,256, 18 for 48, with 5 tokens. Between them by the turns of a CTA, 1,200
+// cycles for 4,096 logits: 333 rows of 50,257 bfloat16 logits (33 MB, 5.1 us) take 18 us without a list and 31 with 20 tokens.
 #include "common.cuh"
 
 #include <type_traits>
@@ -230,7 +231,11 @@ token_logprobs_kernel(const T* __restrict__ logits, long long ld, const int* __r
     const int target = targets[row];
     const bool real = target >= 0 && target < V;
     const float xt = real ? lp_to_float(x[target]) : INFINITY;
-    // A logit comes before the target's if it is larger, and if it is equal and its token lower.
+    // A logit comes before the target's if it is larger, and if it is equal and its token lower: in front of the target it is larger than the
+    // number below the target's. Where the target's is no number, or -inf (which also stands for what is not in the row), logits are looked
+    // at one by one.
+    const bool in_order = !real || xt > -INFINITY;
+    const float below = xt == 0.f ? -__uint_as_float(1u) : __int_as_float(__float_as_int(xt) + (xt > 0.f ? -1 : 1));
 
     Sums s = {-INFINITY, 0.f, 0.f, 0.f, 0};
     uint64_t list = 0, kth = 0;          // the warp's first tokens over its lanes, and the last of the first k
@@ -319,26 +324,22 @@ token_logprobs_kernel(const T* __restrict__ logits, long long ld, const int* __r
         else add_up(std::false_type());
         // the target's rank
         const int at0 = w0 * N - lead;                                // the first logit in the CTA's hands
-        if (__any_sync(ALL, !(most < xt)) || (target >= at0 && target < at0 + PER * THREADS * N)) {
+        if (!in_order) {
 #pragma unroll
-            for (int p = 0; p < PER; ++p) {
-                const int w = w0 + p * THREADS + (int)threadIdx.x, i0 = w * N - lead;
-                // one by one: around the target, against no number, and against -inf where not all are logits of the row
-                if (xt != xt || (i0 <= target && target < i0 + N) || (xt == -INFINITY && !(w >= whole_from && w < whole_to))) {
-                    if (real) {
+            for (int j = 0; j < VALUES; ++j) {
+                const int w = w0 + j / N * THREADS + (int)threadIdx.x, i = w * N - lead + j % N;
+                if (i >= 0 && i < V && w < to && before(v[j], i, xt, target)) ++s.ahead;
+            }
+        } else if (__any_sync(ALL, most >= xt)) {
+            if (at0 > target || at0 + PER * THREADS * N <= target) {
+                const float limit = at0 > target ? xt : below;
 #pragma unroll
-                        for (int e = 0; e < N; ++e)
-                            if (i0 + e >= 0 && i0 + e < V && w < to && before(v[p * N + e], i0 + e, xt, target)) ++s.ahead;
-                    }
-                } else if (i0 < target) {
+                for (int j = 0; j < VALUES; ++j)
+                    if (v[j] > limit) ++s.ahead;
+            } else {
 #pragma unroll
-                    for (int e = 0; e < N; ++e)
-                        if (v[p * N + e] >= xt) ++s.ahead;
-                } else {
-#pragma unroll
-                    for (int e = 0; e < N; ++e)
-                        if (v[p * N + e] > xt) ++s.ahead;
-                }
+                for (int j = 0; j < VALUES; ++j)
+                    if (v[j] > (at0 + (j / N * THREADS + (int)threadIdx.x) * N + j % N < target ? below : xt)) ++s.ahead;
             }
         }
         if (TOP) {

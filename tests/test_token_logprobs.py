@@ -119,6 +119,24 @@ def test_equal_logits_go_by_token(R, V):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("R,V", [(200, 700), (9, 20011)])
+def test_ranks_among_neighbouring_numbers(R, V, dtype):
+    """Zeros of both signs, the numbers next to zero, the largest ones, -inf, and each number's neighbours: the order alone."""
+    info = torch.finfo(dtype)
+    least = info.tiny * 2.0 ** (-23 if dtype == torch.float32 else -7)                     # the smallest number that is not zero
+    one = [1.0, 1.0 + info.eps, 1.0 - info.eps / 2]
+    few = torch.tensor([0.0, -0.0, least, -least, 2 * least, info.max, -info.max, info.tiny, -math.inf] + one + [-v for v in one], dtype=torch.float64).to(dtype)
+    g = torch.Generator().manual_seed(V)
+    x = few[torch.randint(0, len(few), (R, V), generator=g)].cuda()
+    targets = torch.randint(0, V, (R,), generator=g, dtype=torch.int32).cuda()
+    _, _, rank, ids, _ = call(x, targets, 7)
+    want = oracle(x.cpu().float(), targets.cpu(), 7)
+    assert torch.equal(rank.cpu().long(), want[2])
+    assert torch.equal(ids.cpu().long(), want[3])
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("V", [1500, 90001])
 def test_rising_and_falling_rows(V):
     x = torch.stack([torch.linspace(-9, 9, V), torch.linspace(9, -9, V), torch.arange(V).float() % 64, -(torch.arange(V).float() % 640)]).cuda()
