@@ -232,8 +232,8 @@ token_logprobs_kernel(const T* __restrict__ logits, long long ld, const int* __r
     const bool real = target >= 0 && target < V;
     const float xt = real ? lp_to_float(x[target]) : INFINITY;
     // A logit comes before the target's if it is larger, and if it is equal and its token lower: in front of the target it is larger than the
-    // number below the target's. Where the target's is no number, or -inf (which also stands for what is not in the row), logits are looked
-    // at one by one.
+    // number below the target's. -inf has none below and also stands for what is not in the row: in front of it all numbers count, where
+    // all are in the row. One by one only what is left: around such a target, and where the target's logit is no number.
     const bool in_order = !real || xt > -INFINITY;
     const float below = xt == 0.f ? -__uint_as_float(1u) : __int_as_float(__float_as_int(xt) + (xt > 0.f ? -1 : 1));
 
@@ -324,22 +324,29 @@ token_logprobs_kernel(const T* __restrict__ logits, long long ld, const int* __r
         else add_up(std::false_type());
         // the target's rank
         const int at0 = w0 * N - lead;                                // the first logit in the CTA's hands
-        if (!in_order) {
+        const bool behind = at0 > target, in_front = at0 + PER * THREADS * N <= target;
+        if (in_order || (xt == -INFINITY && behind)) {
+            if (__any_sync(ALL, most >= xt)) {
+                if (behind || in_front) {
+                    const float limit = behind ? xt : below;
+#pragma unroll
+                    for (int j = 0; j < VALUES; ++j)
+                        if (v[j] > limit) ++s.ahead;
+                } else {
+#pragma unroll
+                    for (int j = 0; j < VALUES; ++j)
+                        if (v[j] > (at0 + (j / N * THREADS + (int)threadIdx.x) * N + j % N < target ? below : xt)) ++s.ahead;
+                }
+            }
+        } else if (xt == -INFINITY && in_front && w0 >= whole_from && w0 + PER * THREADS <= whole_to) {
+#pragma unroll
+            for (int j = 0; j < VALUES; ++j)
+                if (v[j] == v[j]) ++s.ahead;
+        } else {
 #pragma unroll
             for (int j = 0; j < VALUES; ++j) {
                 const int w = w0 + j / N * THREADS + (int)threadIdx.x, i = w * N - lead + j % N;
                 if (i >= 0 && i < V && w < to && before(v[j], i, xt, target)) ++s.ahead;
-            }
-        } else if (__any_sync(ALL, most >= xt)) {
-            if (at0 > target || at0 + PER * THREADS * N <= target) {
-                const float limit = at0 > target ? xt : below;
-#pragma unroll
-                for (int j = 0; j < VALUES; ++j)
-                    if (v[j] > limit) ++s.ahead;
-            } else {
-#pragma unroll
-                for (int j = 0; j < VALUES; ++j)
-                    if (v[j] > (at0 + (j / N * THREADS + (int)threadIdx.x) * N + j % N < target ? below : xt)) ++s.ahead;
             }
         }
         if (TOP) {

@@ -120,7 +120,7 @@ def test_equal_logits_go_by_token(R, V):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
-@pytest.mark.parametrize("R,V", [(200, 700), (9, 20011)])
+@pytest.mark.parametrize("R,V", [(200, 700), (9, 20011), (450, 20011)])
 def test_ranks_among_neighbouring_numbers(R, V, dtype):
     """Zeros of both signs, the numbers next to zero, the largest ones, -inf, and each number's neighbours: the order alone."""
     info = torch.finfo(dtype)
