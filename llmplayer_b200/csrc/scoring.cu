@@ -15,10 +15,11 @@
 // warps' largest logits so far give. A cluster of CTAs shares a long row when the rows are few; their parts meet in the first CTA's
 // registers through distributed shared memory, so there is no scratch in memory and no order of arrival: results repeat bit for bit.
 //
-// Bound by memory at many rows: 2,000 rows of 128,256 float32 logits (1.03 GB, 157 us at the measured copy rate) take 172 us without
-// a list, 91 %, 184 with the 2 and 197 with the 20 most likely tokens (B200, caches cold): a row's first loads fill the lists of its eight
-// warps. At few rows bound by latency: 14 us for one row of 128,256, 18 for 48, with 5 tokens. Between them by the turns of a CTA, 1,200
-// cycles for 4,096 logits: 333 rows of 50,257 bfloat16 logits (33 MB, 5.1 us) take 18 us without a list and 31 with 20 tokens.
+// Bound by memory at many rows: 2,000 rows of 128,256 float32 logits (1.03 GB, 157 us at the measured copy rate) take 163 us without
+// a list, 96 %, 180 with the most likely token and 211 with the 20 most likely ones (B200, one call behind the other): a row's first loads
+// fill the lists of its eight warps, and its end is nobody's memory time. At few rows bound by latency: 6.6 us for one row of 32,000, 9.5 for 4
+// and 13.5 for 48 of 128,256, with 5 tokens. Between them by the turns of a CTA, 1,200 cycles for 4,096 logits: 333 rows of 50,257
+// bfloat16 logits (33 MB, 5.1 us) take 16 us without a list, 20 with one token and 28 with 20.
 #include "common.cuh"
 
 #include <type_traits>
@@ -276,7 +277,8 @@ token_logprobs_kernel(const T* __restrict__ logits, long long ld, const int* __r
         return __shfl_sync(ALL, post, __ffs(who) - 1);
     };
     float cut = key_value(0);
-    int turn = 0;
+    int turn = 0, again = 0;
+    bool offered = false;
     for (int w0 = from; w0 < to; w0 += PER * THREADS) {
         float v[VALUES];
 #pragma unroll
@@ -351,8 +353,10 @@ token_logprobs_kernel(const T* __restrict__ logits, long long ld, const int* __r
         }
         if (TOP) {
             lane_most = fmaxf(lane_most, most);
-            if ((turn & (turn + 1)) == 0 && (turn == 0 || to - w0 > turn * PER * THREADS)) {
-                // At first, and whenever as much has been seen again as before and most is still to come. Posts only rise, so an old one
+            if (turn == 0 || (offered && turn >= again)) {
+                again = 2 * turn + 1;
+                offered = false;
+                // At first, and when something was offered since and as much has been seen again as before. Posts only rise, so an old one
                 // holds as well.
                 const uint32_t key = warps_key();
                 volatile uint32_t* const posted = posts;
@@ -364,6 +368,7 @@ token_logprobs_kernel(const T* __restrict__ logits, long long ld, const int* __r
             ++turn;
             uint32_t who = __ballot_sync(ALL, !(most < cut));
             if (who) {
+                offered = true;
                 // The lanes with something to offer lay out what they hold, and the warp goes through two lanes' logits at a time.
                 if (!(most < cut)) {
 #pragma unroll
@@ -543,8 +548,8 @@ extern "C" int lp_token_logprobs(const void* logits, int dtype, long long ld, co
     if (rows <= 0 || V <= 0 || top < 0 || top > MOST_TOP || top > V || ld < V || rows > 0x7fffffff / MOST_CLUSTER || V > 0x7fffffff - 4 * THREADS * VALUES)
         LP_REFUSE("token_logprobs: %d rows of %d logits, the %d most likely", rows, V, top);
     // Few rows: as many CTAs per row as the GPU holds at once, each with half a load of its threads at least. B200, 128,256 float32 logits,
-    // 5 tokens, us with 1, 2, 4 and 8 CTAs per row: 1 row 35, 25, 21, 16; 48 rows 37, 27, 25, 23; 100 rows 37, 33, 29, 41;
-    // 220 rows 45, 41, 57, 72; 300 rows 55, 59, 68, 92; 8 rows of 2,000 10, 12, 12, 12; 1 row of 32,000 18, 16, 14, 12.
+    // 5 tokens, us (cold) with 1, 2, 4 and 8 CTAs per row: 1 row 31, 23, 18, 14; 48 rows 33, 25, 21, 21; 100 rows 33, 29, 25, 37;
+    // 220 rows 39, 35, 49, 61; 300 rows 49, 51, 57, 78; 8 rows of 2,000 10, 12, 12, 12; 1 row of 32,000 14, 14, 12, 12.
     int cluster = 1;
     while (cluster < MOST_CLUSTER && (long long)rows * cluster * 2 <= (long long)lp_sm_count() * CTAS_PER_SM && V / (cluster * 2) >= THREADS * VALUES / 2) cluster *= 2;
     if (dtype == LP_F32)
