@@ -1356,7 +1356,7 @@ def attention_shared(q: torch.Tensor, out: torch.Tensor, pages: torch.Tensor, pa
         raise KernelError(f"{what}: at most {max_new} new tokens per sequence")
     if T == 0:
         return out
-    splits, slots = shared_split(T, num_heads, num_kv_heads, int(shared_pages))
+    splits, slots = shared_split(T, num_heads, num_kv_heads, head_dim, int(shared_pages))
     parts = scratch("shared_partials", (slots * T * num_heads * (head_dim + 2),), torch.float32) if slots else None
     part_o = _ptr(parts)
     part_ml = part_o + 4 * slots * T * num_heads * head_dim if slots else None
@@ -1372,18 +1372,20 @@ SHARED_SPLITS_MOST = 32
 
 
 @functools.lru_cache(maxsize=512)
-def shared_split(tokens: int, num_heads: int, num_kv_heads: int, shared_pages: int):
+def shared_split(tokens: int, num_heads: int, num_kv_heads: int, head_dim: int, shared_pages: int):
     """(shares, partial results per row) of the shared pages: a CTA takes two tiles of rows of one key/value head and one share of
     the pages. With a single tile its two chains take alternate pages and leave a result each. The shares are those with the
-    least time in pages of a chain: the last round of CTAs ends after its pages and six for a CTA's start and end, and every result is
-    written and read again at 0.4 of a page. (B200, 32 heads of 128 on 8: 16 sequences on 128 pages 24.5 us with 8 to 10 shares, 28.7 with
-    16; 64 sequences 36.9 with 10 to 18, 41 with 8; 200 sequences on 200 pages 92 with 4, 106 with 3.)"""
+    least time in pages of a chain: the last round of CTAs ends after its pages and six for a CTA's start and end, and a share's results
+    are written and read again at 0.6 of a page per 64 tokens of 32 heads of 128, or 0.4 at least. (B200, 32 heads of 128 on 8: 16 sequences
+    on 128 pages 24.5 us with 8 to 10 shares, 28.7 with 16; 64 sequences 38 with 12 to 18, 42 with 8; 200 sequences on 200 pages 83 with 4, 95
+    with 3, 89 with 9; 4,818 tokens on 150 pages 753 with 1, 761 with 2, 812 with 3; 1,496 tokens on 60 pages 149, 144, 163.)"""
     if shared_pages == 0:
         return 0, 0
     tiles = -(-tokens // (SHARED_ROWS // (num_heads // num_kv_heads)))
     ctas, sms, chains = -(-tiles // 2) * num_kv_heads, num_sms(), 2 if tiles == 1 else 1
+    results = max(0.4, 0.6 * tokens * num_heads * head_dim / (64 * 32 * 128))
     best = min(range(1, min(shared_pages, SHARED_SPLITS_MOST) + 1),
-               key=lambda n: (-(-ctas * n // sms) * (-(-shared_pages // (n * chains)) + 6) + 0.4 * n * chains, n))
+               key=lambda n: (-(-ctas * n // sms) * (-(-shared_pages // (n * chains)) + 6) + results * n * chains, n))
     return best, best * chains
 
 
