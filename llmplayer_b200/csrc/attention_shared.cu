@@ -688,14 +688,17 @@ attention_own_single_kernel(const __grid_constant__ CUtensorMap map_kv, const Ow
 }
 
 // Several new tokens: 64 rows of (token, query head) pairs of one sequence, 16 per warp, over its own pages, causal. These are few next
-// to the shared ones, so mma.sync does; at 40 sequences of up to 190 tokens above it takes 99 us, 5 % of the call, and half of what it
-// moves are the shared pages' results (77 MB).
+// to the shared ones, so mma.sync does. Bound by latency: lengths, page numbers, tiles, then the shared pages' results (each of a row's two
+// rounds of values asked for at once: 4 sequences of 20 tokens behind 30 shared pages 16.4 us in all, 20.7 row by row). Three CTAs per SM:
+// two with registers to spare took 41.8 instead of 35.9 us for 100 sequences of 2 tokens. At 40 sequences of up to 190 tokens above it
+// takes 99 us, 5 % of the call, and most of what it moves are the shared pages' results (77 MB); to take those first, while the pages
+// are on their way, gained nothing there and cost 5 us where the first kernel leaves SMs free.
 // grid: (row tiles, G, B); 128 threads.
 template <int HD> struct OwnRows {
     static constexpr int STAGE = 2 * PAGE * HD * 2, STAGES = 2, SMEM = STAGES * STAGE + 1024;
 };
 template <int HD>
-__global__ void __launch_bounds__(128)
+__global__ void __launch_bounds__(128, 3)
 attention_own_rows_kernel(const __grid_constant__ CUtensorMap map_kv, const OwnArgs a) {
     using SH = OwnRows<HD>;
     constexpr int KSTEPS = HD / 16, STAGES = SH::STAGES;
@@ -746,7 +749,7 @@ attention_own_rows_kernel(const __grid_constant__ CUtensorMap map_kv, const OwnA
     float o[KSTEPS * 2][4];
 #pragma unroll
     for (int i = 0; i < KSTEPS * 2; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-    float m[2] = {NEG_BIG, NEG_BIG}, l[2] = {0.f, 0.f};
+    float m[2] = {NEG_BIG, NEG_BIG}, l[2] = {0.f, 0.f};             // the sum: a part in each of a row's four lanes
     for (int p = 0; p < npages; ++p) {
         uint8_t* stage = smem + (p % STAGES) * SH::STAGE;
         const bool arrived = mbar_wait(&full[p % STAGES], (p / STAGES) & 1);
@@ -824,51 +827,62 @@ attention_own_rows_kernel(const __grid_constant__ CUtensorMap map_kv, const OwnA
             request_page<HD>(stage, &full[p % STAGES], &map_kv, table[p + STAGES], a.G, g);
         }
     }
-    if (!a.waits_first) lp_grid_wait();                            // the shared pages' results
+    // what the shared pages gave
+    if (!a.waits_first) lp_grid_wait();
     lp_grid_release();
-    float own[2], most[2], sum[2];
     const float* po[2];
     const float* ml[2];
     const long long row_step = (long long)a.T * a.H;
+    float f[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        const long long row = (long long)token[k] * a.H + head[k];
+        po[k] = a.part_o + row * HD + t4 * 2;
+        ml[k] = a.part_ml + row * 2;
+        float most = m[k];
+#pragma unroll 2
+        for (int s = t4; s < a.slots; s += 4) {                    // the row's four lanes share them
+            const float2 x = __ldcg(reinterpret_cast<const float2*>(ml[k] + s * row_step * 2));
+            if (x.y != 0.f) most = fmaxf(most, x.x);
+        }
+        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
+        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+        f[k] = fast_exp2(m[k] - most);
+        m[k] = most;
+        l[k] *= f[k];
+    }
+#pragma unroll
+    for (int i = 0; i < KSTEPS * 2; ++i) { o[i][0] *= f[0]; o[i][1] *= f[0]; o[i][2] *= f[1]; o[i][3] *= f[1]; }
+    for (int s = 0; s < a.slots; ++s) {                            // both rows' values asked for together
+        float2 x[2], v[2][KSTEPS * 2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            x[k] = __ldcg(reinterpret_cast<const float2*>(ml[k] + s * row_step * 2));
+#pragma unroll
+            for (int i = 0; i < KSTEPS * 2; ++i) v[k][i] = __ldcg(reinterpret_cast<const float2*>(po[k] + s * row_step * HD + i * 8));
+        }
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            if (x[k].y == 0.f) continue;                           // nothing there
+            const float weight = fast_exp2(x[k].x - m[k]);
+            if (t4 == 0) l[k] += x[k].y * weight;
+#pragma unroll
+            for (int i = 0; i < KSTEPS * 2; ++i) {
+                o[i][2 * k] += v[k][i].x * weight;
+                o[i][2 * k + 1] += v[k][i].y * weight;
+            }
+        }
+    }
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
         l[k] += __shfl_xor_sync(0xffffffffu, l[k], 1);
         l[k] += __shfl_xor_sync(0xffffffffu, l[k], 2);
-        const long long row = (long long)token[k] * a.H + head[k];
-        po[k] = a.part_o + row * HD;
-        ml[k] = a.part_ml + row * 2;
-        most[k] = m[k];
-        for (int s = 0; s < a.slots; ++s) {
-            const float2 x = __ldcg(reinterpret_cast<const float2*>(ml[k] + s * row_step * 2));
-            if (x.y != 0.f) most[k] = fmaxf(most[k], x.x);
-        }
-        own[k] = fast_exp2(m[k] - most[k]);
-        sum[k] = l[k] * own[k];
-    }
-#pragma unroll
-    for (int i = 0; i < KSTEPS * 2; ++i) { o[i][0] *= own[0]; o[i][1] *= own[0]; o[i][2] *= own[1]; o[i][3] *= own[1]; }
-    for (int s = 0; s < a.slots; ++s)
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            const float2 x = __ldcg(reinterpret_cast<const float2*>(ml[k] + s * row_step * 2));
-            if (x.y == 0.f) continue;                              // nothing there
-            const float f = fast_exp2(x.x - most[k]);
-            sum[k] += x.y * f;
-#pragma unroll
-            for (int i = 0; i < KSTEPS * 2; ++i) {
-                const float2 v = __ldcg(reinterpret_cast<const float2*>(po[k] + s * row_step * HD + i * 8 + t4 * 2));
-                o[i][2 * k] += v.x * f;
-                o[i][2 * k + 1] += v.y * f;
-            }
-        }
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-        const float inv = sum[k] != 0.f ? 1.0f / sum[k] : 0.f;
+        const float inv = l[k] != 0.f ? 1.0f / l[k] : 0.f;
         if (real[k]) {
             __nv_bfloat16* dst = a.out + ((long long)token[k] * a.H + head[k]) * HD + t4 * 2;
 #pragma unroll
             for (int i = 0; i < KSTEPS * 2; ++i)
-                *reinterpret_cast<uint32_t*>(dst + i * 8) = sum[k] != 0.f ? pack_bf16(o[i][2 * k] * inv, o[i][2 * k + 1] * inv) : 0u;
+                *reinterpret_cast<uint32_t*>(dst + i * 8) = l[k] != 0.f ? pack_bf16(o[i][2 * k] * inv, o[i][2 * k + 1] * inv) : 0u;
         }
     }
 }
