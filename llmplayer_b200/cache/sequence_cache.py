@@ -17,6 +17,7 @@ its recurrent architectures live in per-request objects too
 """
 from __future__ import annotations
 
+import bisect
 from dataclasses import dataclass
 from typing import Dict, List, Optional, Sequence, Tuple
 
@@ -221,7 +222,7 @@ class SequenceCache:
 
     def shared_pages(self, slots: Sequence[int]) -> List[int]:
         """Per group: how many first pages the slots have in common (0 where pages are given back behind a window or a chunk, and for
-        a single slot)."""
+        a single slot). Slots share pages through forks only, and then all pages in front of a shared one."""
         out = []
         for group in self.groups:
             if len(slots) < 2 or group.pages.window is not None or group.pages.chunk is not None:
@@ -231,12 +232,11 @@ class SequenceCache:
             common = min(len(first), min(self._length[s] for s in slots) // PAGE_SIZE)
             for s in slots[1:]:
                 table = group.pages.table(s)
-                if not common or not table or table[0] != first[0]:
-                    common = 0
-                    break
                 common = min(common, len(table))
-                if table[:common] != first[:common]:
-                    common = next(i for i in range(common) if table[i] != first[i])
+                if common and table[common - 1] != first[common - 1]:
+                    common = bisect.bisect_left(range(common), True, key=lambda i: table[i] != first[i])
+                if not common:
+                    break
             out.append(common)
         return out
 

@@ -237,6 +237,7 @@ attention_shared_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
 #pragma unroll
             for (int c = 0; c < 2; ++c)
                 if (ok && k < counts[c]) request(k, c, 0);
+#pragma unroll 4
         for (int b = lane; b < a.B; b += 32) reached = max(reached, a.kv_len[b]);
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) reached = max(reached, __shfl_xor_sync(0xffffffffu, reached, o));

@@ -150,6 +150,41 @@ def test_no_slot_or_page_is_lost_under_forks():
     assert c.free_pages() == [40] * 3
 
 
+def test_common_pages_are_found_under_random_forks():
+    rng = random.Random(3)
+    c = make_cache(max_tokens=64 * 200, max_slots=30)
+    held = [c.acquire()]
+    for _ in range(1500):
+        op, s = rng.random(), rng.choice(held)
+        try:
+            if op < 0.1:
+                held.append(c.acquire())
+            elif op < 0.4:
+                held += c.fork(s, rng.randint(0, 3))
+            elif op < 0.55 and len(held) > 1:
+                held.remove(s)
+                c.release(s)
+            else:
+                n = rng.randint(1, 150)
+                c.reserve([s], [n])
+                c.commit([s], [n])
+        except CacheFull:
+            for s in held[len(held) // 2:]:
+                c.release(s)
+            held = held[:len(held) // 2]
+        slots = rng.sample(held, rng.randint(1, len(held)))
+        shortest = min(c.length(s) for s in slots) // PAGE_SIZE
+        for g, found in enumerate(c.shared_pages(slots)):
+            tables = [c.groups[g].pages.table(s) for s in slots]
+            if len(slots) < 2 or c.groups[g].pages.window is not None:
+                assert found == 0
+                continue
+            want = 0
+            while want < shortest and len({t[want] for t in tables}) == 1:
+                want += 1
+            assert found == want
+
+
 class ScriptedBackend:
     """Chooses token 10 * slot + step; says so with a log probability."""
 
