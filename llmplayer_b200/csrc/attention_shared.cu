@@ -12,11 +12,11 @@
 //                  begin before the first kernel's results are there (programmatic launch), as far as the SMs have room.
 //
 // B200, 32 query heads on 8, caches cold, the whole call in a graph, against attention that reads every sequence's pages:
-//   64 single tokens, heads of 128, 128 shared pages, up to 250 own positions each: 39 us against 432; the two kernels by
+//   64 single tokens, heads of 128, 128 shared pages, up to 250 own positions each: 37 us against 432; the two kernels by
 //       themselves 21 and 15 us for 70 MB (10.8 us at the measured copy rate).
-//   24 sequences of 9 to 37 tokens, heads of 64, 50 shared pages: 43 against 234; 32 and 13 us for 15 GFLOP.
-//   40 sequences of 47 to 190 tokens, heads of 128, 500 shared pages: 1,890 against 5,390, 1,298 TFLOP/s, 80 % of the measured rate of
-//       dense products (99 us of it the second kernel); 2,100 over a long run, where the power limit holds the clock down.
+//   24 sequences of 9 to 37 tokens, heads of 64, 50 shared pages: 43 against 231; 33 and 12 us for 15 GFLOP.
+//   40 sequences of 47 to 190 tokens, heads of 128, 500 shared pages: 1,890 against 5,380, 1,298 TFLOP/s, 80 % of the measured rate of
+//       dense products (96 us of it the second kernel); 2,100 over a long run, where the power limit holds the clock down.
 //
 // All sums, maxima and partial results are float32. The softmax weights enter the products with the values as bfloat16, rounded
 // against a reference maximum (as in the other attention kernels here); the row sums use the float32 weights.
@@ -692,7 +692,7 @@ attention_own_single_kernel(const __grid_constant__ CUtensorMap map_kv, const Ow
 // to the shared ones, so mma.sync does. Bound by latency: lengths, page numbers, tiles, then the shared pages' results (each of a row's two
 // rounds of values asked for at once: 4 sequences of 20 tokens behind 30 shared pages 16.4 us in all, 20.7 row by row). Three CTAs per SM:
 // two with registers to spare took 41.8 instead of 35.9 us for 100 sequences of 2 tokens. At 40 sequences of up to 190 tokens above it
-// takes 99 us, 5 % of the call, and most of what it moves are the shared pages' results (77 MB); to take those first, while the pages
+// takes 96 us, 5 % of the call, and most of what it moves are the shared pages' results (77 MB); to take those first, while the pages
 // are on their way, gained nothing there and cost 5 us where the first kernel leaves SMs free.
 // grid: (row tiles, G, B); 128 threads.
 template <int HD> struct OwnRows {
