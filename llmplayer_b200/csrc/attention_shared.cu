@@ -9,7 +9,8 @@
 //                  per key head that is 256 rows on one read of the keys, instead of 64 reads. Tensor memory, tcgen05.
 //   own pages      One kernel per step form (a single token per sequence, several tokens) takes the sequence's own pages with
 //                  mma.sync, then joins its result with what the first kernel left in float32. Its reads of its own pages
-//                  begin before the first kernel's results are there (programmatic launch), as far as the SMs have room.
+//                  begin before the first kernel's results are there (programmatic launch), as far as the SMs have room. Few rows of
+//                  several tokens have many results, which a third kernel joins.
 //
 // B200, 32 query heads on 8, caches cold, the whole call in a graph, against attention that reads every sequence's pages:
 //   64 single tokens, heads of 128, 128 shared pages, up to 250 own positions each: 37 us against 432; the two kernels by
@@ -452,8 +453,8 @@ struct OwnArgs {
     int width;
     const int* q_start;
     const int* kv_len;
-    const float* part_o;
-    const float* part_ml;
+    float* part_o;
+    float* part_ml;
     int B, T, H, G, R, pages, slots;           // slots: partial results per row from the shared pages
     int waits_first;                           // nothing runs before it that would have waited
     float scale_log2;
@@ -698,7 +699,8 @@ attention_own_single_kernel(const __grid_constant__ CUtensorMap map_kv, const Ow
 template <int HD> struct OwnRows {
     static constexpr int STAGE = 2 * PAGE * HD * 2, STAGES = 2, SMEM = STAGES * STAGE + 1024;
 };
-template <int HD>
+// APART: the results go behind the shared pages', for the kernel below.
+template <int HD, bool APART>
 __global__ void __launch_bounds__(128, 3)
 attention_own_rows_kernel(const __grid_constant__ CUtensorMap map_kv, const OwnArgs a) {
     using SH = OwnRows<HD>;
@@ -828,6 +830,22 @@ attention_own_rows_kernel(const __grid_constant__ CUtensorMap map_kv, const OwnA
             request_page<HD>(stage, &full[p % STAGES], &map_kv, table[p + STAGES], a.G, g);
         }
     }
+    if (APART) {
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            l[k] += __shfl_xor_sync(0xffffffffu, l[k], 1);
+            l[k] += __shfl_xor_sync(0xffffffffu, l[k], 2);
+            if (!real[k]) continue;
+            const long long row = ((long long)a.slots * a.T + token[k]) * a.H + head[k];
+            if (t4 == 0) *reinterpret_cast<float2*>(a.part_ml + row * 2) = make_float2(m[k], l[k]);
+#pragma unroll
+            for (int i = 0; i < KSTEPS * 2; ++i)
+                *reinterpret_cast<float2*>(a.part_o + row * HD + i * 8 + t4 * 2) = make_float2(o[i][2 * k], o[i][2 * k + 1]);
+        }
+        lp_grid_wait();
+        lp_grid_release();
+        return;
+    }
     // what the shared pages gave
     if (!a.waits_first) lp_grid_wait();
     lp_grid_release();
@@ -888,6 +906,56 @@ attention_own_rows_kernel(const __grid_constant__ CUtensorMap map_kv, const OwnA
     }
 }
 
+// Many results per row and few rows: all of a row's results, the own pages' last, joined by a thread per four features. In the kernel above,
+// whose CTAs are as few as the rows, a result costs a round trip each.
+// grid: rows of (token, query head) in portions of 128 / (HD / 4); 128 threads.
+template <int HD>
+__global__ void __launch_bounds__(128)
+attention_join_kernel(const OwnArgs a) {
+    constexpr int LANES = HD / 4, PER = (MOST_SLOTS + 1 + LANES - 1) / LANES;
+    const int lane = threadIdx.x % LANES;
+    const long long row = (long long)blockIdx.x * (128 / LANES) + threadIdx.x / LANES, step = (long long)a.T * a.H;
+    lp_grid_wait();
+    lp_grid_release();
+    const bool real = row < (long long)min(a.T, a.q_start[a.B]) * a.H;       // rows behind the last sequence stay as they are
+    const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + (real ? row : 0);
+    float2 x[PER];
+    float m = NEG_BIG, l = 0.f;
+#pragma unroll
+    for (int k = 0; k < PER; ++k) x[k] = k * LANES + lane <= a.slots ? __ldcg(ml + (k * LANES + lane) * step) : make_float2(NEG_BIG, 0.f);
+#pragma unroll
+    for (int k = 0; k < PER; ++k) m = fmaxf(m, x[k].y != 0.f ? x[k].x : NEG_BIG);        // nothing lies where the sum is zero
+#pragma unroll
+    for (int o = LANES / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    float factor[PER];
+#pragma unroll
+    for (int k = 0; k < PER; ++k) {
+        factor[k] = x[k].y != 0.f ? fast_exp2(x[k].x - m) : 0.f;
+        l += x[k].y * factor[k];
+    }
+#pragma unroll
+    for (int o = LANES / 2; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+    const float4* po = reinterpret_cast<const float4*>(a.part_o) + (real ? row : 0) * LANES + lane;
+    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int k = 0; k < PER; ++k)
+        for (int j = 0; j < LANES && k * LANES + j <= a.slots; j += 8) {
+            float4 v[8];
+            float f[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                f[u] = __shfl_sync(0xffffffffu, factor[k], j + u, LANES);
+                v[u] = f[u] != 0.f ? __ldcg(po + (long long)(k * LANES + j + u) * step * LANES) : make_float4(0.f, 0.f, 0.f, 0.f);
+            }
+#pragma unroll
+            for (int u = 0; u < 8; ++u) { sum.x += v[u].x * f[u]; sum.y += v[u].y * f[u]; sum.z += v[u].z * f[u]; sum.w += v[u].w * f[u]; }
+        }
+    const float inv = l != 0.f ? 1.0f / l : 0.f;
+    if (real)
+        *reinterpret_cast<uint2*>(a.out + row * HD + lane * 4) =
+            l != 0.f ? make_uint2(pack_bf16(sum.x * inv, sum.y * inv), pack_bf16(sum.z * inv, sum.w * inv)) : make_uint2(0, 0);
+}
+
 // ============================================================================ launches
 int make_query_map(CUtensorMap* map, const void* q, int T, int H, int hd, int R, int tokens) {
     EncodeTiled enc = encode_fn();
@@ -909,12 +977,13 @@ template <typename K> int reserve(K kernel, int bytes) {
 }
 
 template <int HD>
-int run(const void* q, const void* pages, long long num_pages, int max_new, SharedArgs s, OwnArgs o, cudaStream_t stream) {
+int run(const void* q, const void* pages, long long num_pages, int max_new, bool apart, SharedArgs s, OwnArgs o, cudaStream_t stream) {
     static bool configured = false;
     if (!configured) {
         int rc = reserve(attention_shared_kernel<HD>, Shape<HD>::SMEM);
         if (!rc) rc = reserve(attention_own_single_kernel<HD>, OwnShape<HD>::SMEM);
-        if (!rc) rc = reserve(attention_own_rows_kernel<HD>, OwnRows<HD>::SMEM);
+        if (!rc) rc = reserve(attention_own_rows_kernel<HD, false>, OwnRows<HD>::SMEM);
+        if (!rc) rc = reserve(attention_own_rows_kernel<HD, true>, OwnRows<HD>::SMEM);
         if (rc) return rc;
         configured = true;
     }
@@ -932,7 +1001,16 @@ int run(const void* q, const void* pages, long long num_pages, int max_new, Shar
         const int groups = (s.R + HEAD_ROWS - 1) / HEAD_ROWS;
         lp_launch(attention_own_single_kernel<HD>, dim3(s.G * groups, s.B), dim3(128), OwnShape<HD>::SMEM, stream, mkv, o);
     } else {
-        lp_launch(attention_own_rows_kernel<HD>, dim3((unsigned)(((long long)max_new * s.R + 63) / 64), s.G, s.B), dim3(128), OwnRows<HD>::SMEM, stream, mkv, o);
+        const dim3 grid((unsigned)(((long long)max_new * s.R + 63) / 64), s.G, s.B);
+        if (!apart) {
+            lp_launch(attention_own_rows_kernel<HD, false>, grid, dim3(128), OwnRows<HD>::SMEM, stream, mkv, o);
+        } else {
+            lp_launch(attention_own_rows_kernel<HD, true>, grid, dim3(128), OwnRows<HD>::SMEM, stream, mkv, o);
+            rc = lp_check_launch("attention_shared");
+            if (rc) return rc;
+            const long long rows = 128 / (HD / 4);
+            lp_launch(attention_join_kernel<HD>, dim3((unsigned)(((long long)s.T * s.H + rows - 1) / rows)), dim3(128), 0, stream, o);
+        }
     }
     return lp_check_launch("attention_shared");
 }
@@ -942,9 +1020,10 @@ int run(const void* q, const void* pages, long long num_pages, int max_new, Shar
 // q, out: bf16 [T, H, hd]; pages bf16 [num_pages, 2, G, 64, hd]; table int32 [B, width], whose first shared_pages columns are
 // the same in every row; q_start int32 [B + 1]; kv_len int32 [B], lengths with the new tokens, at most max_new of which a sequence
 // has. splits: into how many CTAs the shared pages are cut (0: there is nothing for them); part_o, part_ml float32 [slots, T, H, hd] and
-// [slots, T, H, 2] with slots = splits, or 2 splits if the tokens fill one tile of rows (T <= 128 / (H / G)).
+// [slots, T, H, 2] with slots = splits, or 2 splits if the tokens fill one tile of rows (T <= 128 / (H / G)), and room for one more if the
+// own pages' results are to be joined `apart`.
 extern "C" int lp_attention_shared(const void* q, void* out, const void* pages, long long num_pages, const int* table, int width, const int* q_start,
-                                   const int* kv_len, int B, int T, int max_new, int H, int G, int hd, int shared_pages, float scale, int splits,
+                                   const int* kv_len, int B, int T, int max_new, int H, int G, int hd, int shared_pages, float scale, int splits, int apart,
                                    float* part_o, float* part_ml, int* status, cudaStream_t stream) {
     if (B <= 0 || T <= 0 || max_new <= 0 || G <= 0 || H <= 0 || H % G || H / G > ROWS || (hd != 64 && hd != 128) || shared_pages < 0 || shared_pages > width)
         LP_REFUSE("attention_shared: %d sequences, %d tokens, %d heads on %d of %d, %d shared pages", B, T, H, G, hd, shared_pages);
@@ -957,5 +1036,5 @@ extern "C" int lp_attention_shared(const void* q, void* out, const void* pages, 
     SharedArgs s = {(const __nv_bfloat16*)pages, num_pages, table, q_start, kv_len, part_o, part_ml, B, T, H, G, R, shared_pages, splits > 0 ? splits : 1, scale * LOG2E, status};
     OwnArgs o = {(const __nv_bfloat16*)q, (__nv_bfloat16*)out, table, width, q_start, kv_len, part_o, part_ml, B, T, H, G, R, shared_pages,
                  one_tile ? 2 * splits : splits, splits == 0, scale * LOG2E, status};
-    return hd == 64 ? run<64>(q, pages, num_pages, max_new, s, o, stream) : run<128>(q, pages, num_pages, max_new, s, o, stream);
+    return hd == 64 ? run<64>(q, pages, num_pages, max_new, apart && splits > 0, s, o, stream) : run<128>(q, pages, num_pages, max_new, apart && splits > 0, s, o, stream);
 }

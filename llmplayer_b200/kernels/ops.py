@@ -148,7 +148,7 @@ _SIGNATURES = {
         "lp_copy_pages": [_P, _I, ctypes.c_longlong, ctypes.c_longlong, _P, _I, _P],
     },
     "attention_shared": {
-        "lp_attention_shared": [_P, _P, _P, ctypes.c_longlong, _P, _I, _P, _P, _I, _I, _I, _I, _I, _I, _I, _F, _I, _P, _P, _P, _P],
+        "lp_attention_shared": [_P, _P, _P, ctypes.c_longlong, _P, _I, _P, _P, _I, _I, _I, _I, _I, _I, _I, _F, _I, _I, _P, _P, _P, _P],
     },
 }
 
@@ -1357,18 +1357,24 @@ def attention_shared(q: torch.Tensor, out: torch.Tensor, pages: torch.Tensor, pa
     if T == 0:
         return out
     splits, slots = shared_split(T, num_heads, num_kv_heads, head_dim, int(shared_pages))
-    parts = scratch("shared_partials", (slots * T * num_heads * (head_dim + 2),), torch.float32) if slots else None
+    apart = int(max_new) > 1 and slots >= SHARED_JOIN_APART
+    room = (slots + apart) * T * num_heads
+    parts = scratch("shared_partials", (room * (head_dim + 2),), torch.float32) if slots else None
     part_o = _ptr(parts)
-    part_ml = part_o + 4 * slots * T * num_heads * head_dim if slots else None
+    part_ml = part_o + 4 * room * head_dim if slots else None
     lib = library("attention_shared")
     _check(lib, lib.lp_attention_shared(q.data_ptr(), out.data_ptr(), pages.data_ptr(), cache[0], page_table.data_ptr(), table[1],
                                         q_start.data_ptr(), kv_len.data_ptr(), B, T, int(max_new), num_heads, num_kv_heads, head_dim, int(shared_pages),
-                                        float(scale), splits, part_o, part_ml, kernel_status().data_ptr(), _stream()))
+                                        float(scale), splits, apart, part_o, part_ml, kernel_status().data_ptr(), _stream()))
     return out
 
 
 SHARED_ROWS = 128             # (token, query head) rows of a tile of the shared pages' products
 SHARED_SPLITS_MOST = 32
+# Several tokens: from so many results per row on a kernel of its own joins them and the own pages'. B200, in the own pages' kernel against
+# apart, us: 30 tokens of 32 heads of 128 on 64 pages (16 results) 38.9 against 20.0, 131 tokens (6) 44.0 against 26.5, 257 tokens (3) 42.4
+# against 37.2; heads of 64: 588 tokens (3) 53.3 against 53.5, 571 tokens on 50 pages (2) 34.6 against 37.0.
+SHARED_JOIN_APART = 3
 
 
 @functools.lru_cache(maxsize=512)
