@@ -1312,10 +1312,11 @@ def attention_shared_serves(num_heads: int, num_kv_heads: int, head_dim: int, pa
 
 
 # From how many pages read over again (sequences times shared pages) on the shared form is used: 256 for a step of single tokens, whose
-# other form rotates, stores and attends in one kernel, 64 for several tokens. B200, 32 heads on 8, shared against ordinary attention alone:
-# single tokens, heads of 64: 8 sequences on 32 pages 18.4 against 26.6 us, on 16 pages 14.3 against 18.4; 64 on 4 14.3 against 16.4;
-# 24 tokens each: 2 sequences on 32 pages 24.6 against 41 us, on 16 22.5 against 24.5; 8 on 8 18.4 against 20.4, on 4 18.4 against 16.4.
-SHARED_PAGES_SINGLE, SHARED_PAGES_SEVERAL = 256, 64
+# other form rotates, stores and attends in one kernel, 32 for several tokens. B200, 32 heads on 8, shared against ordinary attention alone:
+# single tokens, heads of 64: 8 sequences on 32 pages 18.4 against 28.5 us, on 16 pages 16.4 against 20.5; 64 on 4 18.4 against 16.4;
+# 24 tokens each, heads of 64 and of 128: 2 sequences on 16 pages 20.5 against 24.6 and 20.5 against 34.8, on 8 18.4 against 16.4 and 22.5;
+# 4 on 8 18.4 against 18.4 and 20.5 against 24.6, on 4 18.4 against 14.3 and 22.5 against 18.4; 8 on 4 18.4 against 16.4 and 26.6 against 24.6.
+SHARED_PAGES_SINGLE, SHARED_PAGES_SEVERAL = 256, 32
 
 
 def attention_shared_pays(sequences: int, shared_pages: int, single: bool) -> bool:
