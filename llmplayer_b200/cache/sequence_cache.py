@@ -136,6 +136,8 @@ class SequenceCache:
             raise CacheError(f"max_slots must be positive, got {self.max_slots}")
         self.slots = FreeList(self.max_slots, "slot")
         self._length: Dict[int, int] = {}
+        self._birth: Dict[int, int] = {}       # slot -> which of all acquired and forked sequences it holds
+        self._births = 0
         self.groups: List[KVGroup] = []
         self._views: List[object] = [None] * len(requests)
         # every paged request (a run's own, or a member's of a run's bundle) is a leaf with a key of its own
@@ -180,9 +182,14 @@ class SequenceCache:
             self._views[run] = make_view((run,), req)
 
     # ------------------------------------------------------------------ slots
+    def _begin(self, slot: int, length: int) -> None:
+        self._length[slot] = length
+        self._birth[slot] = self._births
+        self._births += 1
+
     def acquire(self) -> int:
         slot = self.slots.take()
-        self._length[slot] = 0
+        self._begin(slot, 0)
         for group in self.groups:
             group.pages.open(slot)
         for rows in self._state_rows:
@@ -204,7 +211,7 @@ class SequenceCache:
                                 f"{group.pages.pool.num_free} of {group.pages.pool.count} are free")
         new = [self.slots.take() for _ in range(count)]
         for s in new:
-            self._length[s] = length
+            self._begin(s, length)
         for group in self.groups:
             copies = [pair for pair in (group.pages.fork(slot, s, length) for s in new) if pair is not None]
             if not copies:
@@ -245,7 +252,7 @@ class SequenceCache:
             raise CacheError(f"slot {slot} is not held (freed twice?)")
         for group in self.groups:
             group.pages.close(slot)
-        del self._length[slot]
+        del self._length[slot], self._birth[slot]
         self.slots.give_back(slot)
 
     def length(self, slot: int) -> int:
@@ -253,6 +260,13 @@ class SequenceCache:
             return self._length[slot]
         except KeyError:
             raise CacheError(f"slot {slot} is not held") from None
+
+    def births(self, slots: Sequence[int]) -> List[int]:
+        """A number per slot that no sequence before it had: a slot that was released and handed out again has another one, though a fork
+        may have given it the same length at once."""
+        for slot in slots:
+            self.length(slot)
+        return [self._birth[slot] for slot in slots]
 
     def view(self, run: int):
         return self._views[run]

@@ -162,7 +162,9 @@ class Engine:
         elif (tables and self.runtime.device.type == "cuda"
               and 2 * len(tokens) + sum(len(t) for group in tables for t in group) >= StepContext.ON_DEVICE_ENTRIES):
             return StepContext(self.workspace, sequences, tokens, tables, rows, shared_pages=shared, on_device=True)
-        return StepContext(self.workspace, sequences, tokens, tables, rows, min_table_width=width, shared_pages=shared)
+        ctx = StepContext(self.workspace, sequences, tokens, tables, rows, min_table_width=width, shared_pages=shared)
+        ctx.births = self.cache.births(slots)
+        return ctx
 
     def run(self, ctx: StepContext) -> torch.Tensor:
         """Run a planned step; returns float32 logits [wanted, vocab] (valid until the next step)."""
@@ -252,6 +254,8 @@ class Engine:
             if not cache.slots.is_held(slot) or cache.length(slot) != pos + 1 or pos + 2 > limit:
                 return None
             tokens.append(tok)
+        if cache.births(last.slot_list) != last.births:
+            return None                         # a slot holds another sequence by now (a fork has its length at once)
         if not advance:
             return last
         slots = last.slot_list
@@ -276,6 +280,8 @@ class Engine:
         for slot, pos in zip(slots, last.first_positions):
             if not self.cache.slots.is_held(slot) or self.cache.length(slot) != pos + 1 or pos + 2 > self.context_length:
                 return
+        if self.cache.births(slots) != last.births:
+            return
         try:
             self.cache.reserve(slots, [1] * len(slots))
         except LLMPlayerError:
