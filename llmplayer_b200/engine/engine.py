@@ -53,6 +53,7 @@ class Engine:
         self._graphs = {}
         self._fused = {}               # captured decode steps with upload, argmax and read-back inside
         self._last_ctx: Optional[StepContext] = None
+        self._sharing_groups = None    # per cache group: whether a run attends over shared pages once for all
         self._prepared = None          # (context, page tables): the next decode step's pages, reserved ahead
         from ..cache.sequence_cache import keeps_state
         # whether a run keeps a state that a step changes in place (running a step twice would change it twice)
@@ -161,10 +162,23 @@ class Engine:
                 width *= 2
         elif (tables and self.runtime.device.type == "cuda"
               and 2 * len(tokens) + sum(len(t) for group in tables for t in group) >= StepContext.ON_DEVICE_ENTRIES):
-            return StepContext(self.workspace, sequences, tokens, tables, rows, shared_pages=shared, on_device=True)
+            ctx = StepContext(self.workspace, sequences, tokens, tables, rows, shared_pages=shared, on_device=True)
+            ctx.shared_pages = self._attended_once(ctx, shared)
+            return ctx
         ctx = StepContext(self.workspace, sequences, tokens, tables, rows, min_table_width=width, shared_pages=shared)
         ctx.births = self.cache.births(slots)
+        ctx.shared_pages = self._attended_once(ctx, shared)
         return ctx
+
+    def _attended_once(self, ctx: StepContext, shared: List[int]) -> List[int]:
+        """Per cache group: the shared pages that the step attends over once for all its sequences; 0 where no run of the group does
+        so or it does not pay. A captured graph is a matter of these alone, and not of how many pages sequences happen to share."""
+        if not any(shared):
+            return shared
+        if self._sharing_groups is None:
+            self._sharing_groups = self.model.groups_sharing_pages(self.cache)
+        return [n if n and reads and ops.attention_shared_pays(ctx.num_sequences, n, ctx.all_single) else 0
+                for n, reads in zip(shared, self._sharing_groups)]
 
     def run(self, ctx: StepContext) -> torch.Tensor:
         """Run a planned step; returns float32 logits [wanted, vocab] (valid until the next step)."""

@@ -12,6 +12,7 @@ from typing import Dict, List, Mapping, Optional
 
 import torch
 
+from ..cache.sequence_cache import BundleView, KVView
 from ..errors import ConfigError
 from ..parts import BLOCKS
 from ..parts.base import Runtime
@@ -98,6 +99,22 @@ class Model:
     def cache_owner(self, run_index: int) -> int:
         ref = self.runs[run_index].reads_cache_of
         return run_index if ref is None else ref
+
+    def groups_sharing_pages(self, cache) -> List[bool]:
+        """Per cache group: whether a run attends over pages that all of a step's sequences begin with once for all of them (its mixer's
+        ``reads_shared_pages``)."""
+        out = [False] * len(cache.groups)
+
+        def look(mixer, view) -> None:
+            if isinstance(view, BundleView):
+                for member, members_view in zip(mixer.children(), view.members):
+                    look(member, members_view)
+            elif isinstance(view, KVView) and hasattr(mixer, "reads_shared_pages") and mixer.reads_shared_pages(view):
+                out[view.group_index] = True
+
+        for i, run in enumerate(self.runs):
+            look(getattr(self.blocks[run.layer], "mixer", None), cache.view(self.cache_owner(i)))
+        return out
 
     # ------------------------------------------------------------------ a step
     def forward(self, ctx, cache, rows: torch.Tensor, logits: torch.Tensor) -> torch.Tensor:

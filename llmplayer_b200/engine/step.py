@@ -136,9 +136,9 @@ class StepContext:
     A context of one token per sequence can be moved on to the next step of the same sequences
     (:meth:`advance`): only the tokens, positions and lengths are copied again.
 
-    ``shared_pages`` per cache group: so many first columns of its page table are the same in every row. ``on_device``: only
-    tokens, lengths and the pages' numbers are copied, shared ones once, and a kernel builds the tables from them
-    (``ops.step_tables``); such a context cannot be moved on.
+    ``shared_pages`` per cache group: so many first columns of its page table are the same in every row (the engine leaves those that the
+    step attends over once for all its sequences). ``on_device``: only tokens, lengths and the pages' numbers are copied, shared ones
+    once, and a kernel builds the tables from them (``ops.step_tables``); such a context cannot be moved on.
     """
 
     # From so many entries of the tables on they are built on the device. On the host an entry costs about 50 ns, the kernel's launch

@@ -1280,13 +1280,13 @@ def attention(ctx, q: torch.Tensor, out: torch.Tensor, pages: torch.Tensor, page
     """Attention of the step's tokens over the cache; picks the kernel for the step's shape. ``keep_first`` (with a
     window): the first tokens of a sequence that stay visible beyond the window. ``chunk``, ``distance``,
     ``gate``: see :func:`attention_plain`. ``shared_pages``: so many first columns of the page table are the same in every row
-    (see :func:`attention_shared`; used where nothing shapes the scores and the kernel is built for the heads)."""
+    (see :func:`attention_shared`; used where nothing shapes the scores and the kernel is built for the heads. Whether it pays is the
+    caller's to say: :func:`attention_shared_pays`)."""
     tensor_cores = (fast and q.dtype == torch.bfloat16 and pages.dtype == torch.bfloat16
                     and head_dim % 16 == 0 and head_dim <= 256)
     keep_first = int(keep_first) if window else 0
     if (tensor_cores and shared_pages and not window and not softcap and sinks is None and not exact_weights and not chunk
-            and distance is None and gate is None and attention_shared_serves(num_heads, num_kv_heads, head_dim, pages.shape[3])
-            and attention_shared_pays(page_table.shape[0], shared_pages, ctx.all_single)):
+            and distance is None and gate is None and attention_shared_serves(num_heads, num_kv_heads, head_dim, pages.shape[3])):
         return attention_shared(q, out, pages, page_table, ctx.q_start, ctx.kv_len, ctx.buffer, shared_pages=shared_pages,
                                 max_new=ctx.max_new, num_heads=num_heads, num_kv_heads=num_kv_heads, head_dim=head_dim, scale=scale)
     if tensor_cores and ctx.all_single:

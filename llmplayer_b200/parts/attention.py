@@ -150,12 +150,17 @@ class Attention(Part):
 
     # ------------------------------------------------------------------ step
     def _shared_pages(self, ctx, cache) -> int:
-        """How many of the cache group's first pages all of the step's sequences share, if it pays to attend over them once."""
-        s = self.spec
+        """How many of the cache group's first pages the step attends over once for all its sequences."""
         n = ctx.shared_pages[cache.group_index]
-        serves = (n > 0 and self.runtime.fast and s.window is None and s.chunk is None and cache.pages.dtype == torch.bfloat16
-                  and ops.attention_shared_serves(s.num_heads, s.num_kv_heads, s.head_dim, cache.pages.shape[3]))
-        return n if serves and ops.attention_shared_pays(ctx.num_sequences, n, ctx.all_single) else 0
+        return n if n and self.reads_shared_pages(cache) else 0
+
+    def reads_shared_pages(self, cache) -> bool:
+        """Whether this part can attend over pages that all of a step's sequences begin with once for all of them: the kernel is built for
+        its heads, and nothing shapes the scores."""
+        s = self.spec
+        return (self.runtime.fast and s.window is None and s.chunk is None and not s.softcap and self.sinks is None and not s.exact_weights
+                and self.distance is None and s.head_gate is None and cache.pages.dtype == torch.bfloat16
+                and ops.attention_shared_serves(s.num_heads, s.num_kv_heads, self.stored_dim, cache.pages.shape[3]))
 
     @property
     def offers_inputs(self) -> bool:
@@ -245,7 +250,7 @@ class Attention(Part):
             ops.attention(ctx, q, o, cache.pages, table, num_heads=H, num_kv_heads=G, head_dim=hd, scale=s.scale,
                           window=s.window, fast=rt.fast, softcap=s.softcap, sinks=self.sinks, exact_weights=s.exact_weights,
                           keep_first=int(s.keep_first or 0), chunk=int(s.chunk or 0), distance=self.distance, gate=gate,
-                          shared_pages=ctx.shared_pages[cache.group_index])
+                          shared_pages=self._shared_pages(ctx, cache))
         with ops.section("attention.out"):
             if overwrite:
                 if clear is not None:

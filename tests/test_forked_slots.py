@@ -19,11 +19,14 @@ class Recorder:
     capture_safe = False
 
     def __init__(self, requests):
-        self.requests, self.seen = requests, []
+        self.requests, self.seen, self.shares = requests, [], True
         self.layout = SimpleNamespace(head=SimpleNamespace(vocab_size=VOCAB))
 
     def cache_requests(self):
         return self.requests
+
+    def groups_sharing_pages(self, cache):
+        return [self.shares] * len(cache.groups)
 
     def forward(self, ctx, cache, rows, logits):
         self.seen.append(([t.tolist() for t in ctx.page_tables], ctx.kv_len.tolist(), ctx.slots.tolist(), ctx.shared_pages))
@@ -110,6 +113,47 @@ def test_a_step_of_the_same_sequences_still_continues():
     for _ in range(20):
         step(eng, [a, b])
         assert eng._last_ctx is ctx
+
+
+def two_on_a_prompt(eng, length):
+    """The description of a step of two forks of a prompt, which are released again."""
+    a = eng.acquire()
+    eng.step([(a, [1] * length)], [[]])
+    slots = [a] + eng.fork(a, 1)
+    step(eng, slots)
+    ctx = eng._last_ctx
+    for s in slots:
+        eng.release(s)
+    return ctx
+
+
+@pytest.mark.parametrize("shares,single", [(False, 1), (True, 10 ** 9), (True, 1)])
+def test_a_graph_depends_on_shared_pages_only_where_they_are_attended_over_once(monkeypatch, shares, single):
+    from llmplayer_b200.kernels import ops
+    monkeypatch.setattr(ops, "SHARED_PAGES_SINGLE", single)
+    eng = engine_on_the_host(requests=(KVRequest(8, 64),))
+    eng.model.shares = shares
+    shapes = {two_on_a_prompt(eng, length).table_shapes for length in (70, 130, 200, 260)}
+    assert shapes == ({((8, n),) for n in (1, 2, 3, 4)} if shares and single == 1 else {((8, 0),)})
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("everywhere,graphs", [(False, 1), (True, 3)])
+def test_graphs_of_forks_of_prompts_of_several_lengths(tmp_path, monkeypatch, everywhere, graphs):
+    from llmplayer_b200.kernels import ops
+    if everywhere:
+        monkeypatch.setattr(ops, "SHARED_PAGES_SINGLE", 1)
+    eng = Engine.load(make_model(tmp_path, "D"), context_length=512, max_batch=4)        # (engines in float32 capture nothing)
+    for length in (130, 200, 260, 140):
+        a = eng.acquire()
+        eng.step([(a, random_tokens(length, eng.vocab_size, seed=length))], [[]])
+        slots = [a] + eng.fork(a, 2)
+        for _ in range(3):
+            eng.step([(s, [3 + s]) for s in slots], [[0]] * 3)
+        for s in slots:
+            eng.release(s)
+    assert len({shapes for _, shapes, _, _ in eng._graphs}) == graphs          # (the buffer of the step's integers moves as it grows, too)
+    eng.check()
 
 
 @pytest.mark.gpu
