@@ -177,8 +177,18 @@ class Engine:
             return shared
         if self._sharing_groups is None:
             self._sharing_groups = self.model.groups_sharing_pages(self.cache)
-        return [n if n and reads and ops.attention_shared_pays(ctx.num_sequences, n, ctx.all_single) else 0
-                for n, reads in zip(shared, self._sharing_groups)]
+        out, single = [], ctx.max_new == 1
+        keys = sum(n * (have + 0.5 * n) for have, n in zip(ctx.first_positions, ctx.new_counts)) / ctx.num_tokens      # that a token sees, in the mean
+        for n, group, reads in zip(shared, self.cache.groups, self._sharing_groups):
+            if n and reads:
+                heads = group.request.num_kv_heads, group.request.head_dim
+                own = -(-ctx.max_kv_len // PAGE_SIZE) - n if single else max(0.0, keys / PAGE_SIZE - n)
+                if not ops.attention_shared_pays(ctx.num_sequences, n, ctx.max_new, own, *heads):
+                    n = 0
+                elif single:
+                    ctx.shared_until = min(ctx.shared_until, PAGE_SIZE * (n + ops.attention_shared_reach(ctx.num_sequences, n, *heads) // 1))
+            out.append(n if reads else 0)
+        return out
 
     def run(self, ctx: StepContext) -> torch.Tensor:
         """Run a planned step; returns float32 logits [wanted, vocab] (valid until the next step)."""
@@ -270,6 +280,8 @@ class Engine:
             tokens.append(tok)
         if cache.births(last.slot_list) != last.births:
             return None                         # a slot holds another sequence by now (a fork has its length at once)
+        if last.max_kv_len + 1 > last.shared_until:
+            return None                         # the sequences' own pages have become too many for the way their shared ones are attended over
         if not advance:
             return last
         slots = last.slot_list

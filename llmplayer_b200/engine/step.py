@@ -10,6 +10,7 @@ to the device in one copy.
 """
 from __future__ import annotations
 
+import math
 from dataclasses import dataclass
 from typing import Dict, List, Optional, Sequence, Tuple
 
@@ -164,6 +165,7 @@ class StepContext:
         self.wanted_rows = list(wanted_rows)
         # one token for each sequence and every sequence's logits wanted: the shape a decode step continues in
         self.continues_all = self.all_single and self.wanted_rows == list(range(B))
+        self.shared_until = math.inf      # set by the engine: up to which length its choice of shared pages holds
         self.shared_pages = list(shared_pages) if shared_pages is not None else [0] * len(page_tables)
         if on_device:
             self.continues_all = False

@@ -1311,16 +1311,41 @@ def attention_shared_serves(num_heads: int, num_kv_heads: int, head_dim: int, pa
             and num_heads // num_kv_heads <= 128)
 
 
-# From how many pages read over again (sequences times shared pages) on the shared form is used: 256 for a step of single tokens, whose
-# other form rotates, stores and attends in one kernel, 32 for several tokens. B200, 32 heads on 8, shared against ordinary attention alone:
-# single tokens, heads of 64: 8 sequences on 32 pages 18.4 against 28.5 us, on 16 pages 16.4 against 20.5; 64 on 4 18.4 against 16.4;
-# 24 tokens each, heads of 64 and of 128: 2 sequences on 16 pages 20.5 against 24.6 and 20.5 against 34.8, on 8 18.4 against 16.4 and 22.5;
-# 4 on 8 18.4 against 18.4 and 20.5 against 24.6, on 4 18.4 against 14.3 and 22.5 against 18.4; 8 on 4 18.4 against 16.4 and 26.6 against 24.6.
-SHARED_PAGES_SINGLE, SHARED_PAGES_SEVERAL = 256, 32
+# When attending over shared pages once for all pays. Per layer, with against without, on a B200 through the engine (32 heads on 8 of 64 / of 128):
+# Single tokens. The other form rotates, stores and attends in one kernel, and shares a sequence's own pages out over the SMs, where here one CTA goes
+# through them one behind the other: 0.74 us (heads of 64) or 0.89 (128) per page from the fifth on, unless the batch is large enough for its reads to take
+# longer. That and 8 us are set against 0.032 ns for each page, key/value head and feature that is not read again; counted in 64 features, 2 ns:
+#   8 sequences on 128 pages, 4 own pages 59 / 96 us against 61 / 118; 64 own pages 94 / 165 against 70 / 153; 200 own pages 199 / 297 against 90 / 190
+#   64 on 8, 16 own 94 / 168 against 90 / 190; 16 on 32, 4 own 58 / 113 against 57 / 123; 2 on 512, 4 own 71 / 131 against 61 / 139; 200 own 198 / 300 against 68 / 151
+SHARED_PAGES_SINGLE = 3900
+# Several tokens, runs of up to 64: the other form goes through all pages of a sequence one behind the other as well, so shared ones alone are counted:
+#   24 tokens each, none of their own before: 2 sequences on 8 pages 59 / 117 against 64 / 128; 8 on 4 107 / 212 against 103 / 209, on 8 106 / 212 against 109 / 219;
+#   60 on 1 209 / 606 against 242 / 648
+# Longer runs have tcgen05 there, and mma.sync here for the own pages; the shared ones run at 1.3 to 2.5 times the other form's rate. Both go with the tokens, so
+# what counts are a token's keys: its own ones twice, and 1,200 for the results' way, against the shared ones.
+#   8 sequences of 400 tokens on 4 pages 418 / 1,229 against 411 / 1,156, on 64 544 / 1,350 against 601 / 1,506; with 100 own pages on 64 1,071 / 2,334 against 943 / 2,188
+#   and on 256 1,482 / 2,741 against 1,601 / 3,378; 60 of 96 on 4 669 / 2,210 against 666 / 2,012, on 64 883 / 2,381 against 1,011 / 2,681
+SHARED_PAGES_SEVERAL = 40
 
 
-def attention_shared_pays(sequences: int, shared_pages: int, single: bool) -> bool:
-    return sequences > 1 and sequences * shared_pages >= (SHARED_PAGES_SINGLE if single else SHARED_PAGES_SEVERAL)
+def attention_shared_reach(sequences: int, shared_pages: int, num_kv_heads: int, head_dim: int) -> float:
+    """Up to how many own pages of its longest sequence a step of single tokens gains by :func:`attention_shared`; negative: never."""
+    if sequences < 2:
+        return -1.0
+    per_page = num_kv_heads * head_dim / 64                                   # what a sequence reads of a page
+    spare = (sequences - 1.5) * shared_pages * per_page - SHARED_PAGES_SINGLE
+    more = 1.135 * (head_dim + 256) - sequences * per_page                    # an own page, one behind the other against shared out
+    return spare if spare < 0 else float("inf") if more <= 0 else 4 + spare / more
+
+
+def attention_shared_pays(sequences: int, shared_pages: int, max_new: int, own_pages: float, num_kv_heads: int, head_dim: int) -> bool:
+    """Whether a step of so many sequences, of up to ``max_new`` tokens each, gains by :func:`attention_shared`. ``own_pages``: pages behind the
+    shared ones, of the longest sequence for single tokens, else seen by a token in the mean."""
+    if max_new == 1:
+        return own_pages <= attention_shared_reach(sequences, shared_pages, num_kv_heads, head_dim)
+    if max_new <= 64:
+        return sequences > 1 and max(8, sequences) * shared_pages >= SHARED_PAGES_SEVERAL
+    return sequences > 1 and shared_pages >= SHARED_PAGES_SEVERAL * (0.48 + own_pages / 20)
 
 
 def attention_shared(q: torch.Tensor, out: torch.Tensor, pages: torch.Tensor, page_table: torch.Tensor, q_start: torch.Tensor,
