@@ -346,7 +346,8 @@ class Engine:
     def score(self, prompt: Sequence[int], continuations: Sequence[Sequence[int]], *, top: int = 0):
         """The log probability of every token of each continuation of ``prompt`` (both token ids), without sampling: one
         :class:`llmplayer_b200.engine.scoring.ScoredTokens` per continuation, in order. The prompt is run once; the continuations go on
-        from forks of it, as many at a time as the cache has slots and pages for. ``top``: list so many most likely tokens beside each."""
+        from forks of it, as many at a time as the cache has slots and pages for (where it has none for a fork beside the prompt, each is run
+        with the prompt). ``top``: list so many most likely tokens beside each."""
         from .scoring import score
         return score(self, prompt, continuations, top)
 

@@ -116,21 +116,32 @@ def score(engine, prompt: Sequence[int], continuations: Sequence[Sequence[int]],
     if not todo:
         return [ScoredTokens(r) for r in results]
     # the last prompt token runs with each continuation: its logits are the first token's
+    before = prompt[:-1]
     parent = None
     held: List[int] = []
     try:
-        if len(prompt) > 1:
+        if before and len(todo) > 1 and engine.cache.slots.num_free > 1:
             parent = engine.acquire()
-            engine.step([(parent, prompt[:-1])], [[]])
+            engine.step([(parent, before)], [[]])
         while todo:
+            if parent is not None and not engine.forks_fit(parent, [len(conts[todo[0]])]):
+                engine.release(parent)             # no room beside it: the prompt is run with each continuation
+                parent = None
             batch, rows = [], 0
             for i in todo:
-                if batch and (rows + len(conts[i]) > most_rows or not engine.forks_fit(parent, [len(conts[j]) for j in batch + [i]])):
+                more = [len(conts[j]) + (0 if parent is not None else len(before)) for j in batch + [i]]
+                if batch and (rows + len(conts[i]) > most_rows or not engine.forks_fit(parent, more)):
                     break
                 batch.append(i)
                 rows += len(conts[i])
             todo = todo[len(batch):]
-            held = engine.fork(parent, len(batch)) if parent is not None else [engine.acquire() for _ in batch]
+            if parent is not None:
+                held = engine.fork(parent, len(batch))
+            else:
+                for _ in batch:
+                    held.append(engine.acquire())
+                if before:
+                    engine.step([(slot, before) for slot in held], [[]] * len(held))
             runs = [prompt[-1:] + conts[i][:-1] for i in batch]
             # one step, or several if a single continuation has more tokens than a step may have rows of logits
             for a in range(0, max(len(r) for r in runs), most_rows):
