@@ -212,19 +212,25 @@ class SequenceCache:
         new = [self.slots.take() for _ in range(count)]
         for s in new:
             self._begin(s, length)
-        for group in self.groups:
-            copies = [pair for pair in (group.pages.fork(slot, s, length) for s in new) if pair is not None]
-            if not copies:
-                continue
-            sources, targets = [a for a, _ in copies], [b for _, b in copies]
-            if group.storage.is_cuda:
-                ops.copy_pages(group.storage, sources, targets)
-            else:
-                group.storage[:, targets] = group.storage[:, sources]
-        if new and self._state_rows:
-            places = torch.tensor(new, device=self.device)
-            for rows in self._state_rows:
-                rows[places] = rows[slot].clone()
+        try:
+            for group in self.groups:
+                copies = [pair for pair in [group.pages.fork(slot, s, length) for s in new] if pair is not None]
+                if not copies:
+                    continue
+                sources, targets = [a for a, _ in copies], [b for _, b in copies]
+                if group.storage.is_cuda:
+                    ops.copy_pages(group.storage, sources, targets)
+                else:
+                    group.storage[:, targets] = group.storage[:, sources]
+            if new and self._state_rows:
+                places = torch.tensor(new, device=self.device)
+                for rows in self._state_rows:
+                    rows[places] = rows[slot].clone()
+        except BaseException:
+            # a copy failed (the storage lies on another device than the current one, memory ran out): the new slots go back
+            for s in new:
+                self.release(s)
+            raise
         return new
 
     def shared_pages(self, slots: Sequence[int]) -> List[int]:
@@ -251,7 +257,8 @@ class SequenceCache:
         if not self.slots.is_held(slot):
             raise CacheError(f"slot {slot} is not held (freed twice?)")
         for group in self.groups:
-            group.pages.close(slot)
+            if group.pages.holds(slot):
+                group.pages.close(slot)
         del self._length[slot], self._birth[slot]
         self.slots.give_back(slot)
 

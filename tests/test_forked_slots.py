@@ -212,3 +212,27 @@ def test_the_better_of_two_is_kept_and_forked_again(tmp_path, dtype, way):
         eng.release(s)
     eng.check()
     assert eng.cache.free_pages() == [eng.cache.num_pages]
+
+
+def test_a_fork_whose_copies_fail_leaves_nothing_held(monkeypatch):
+    eng = engine_on_the_host(requests=(KVRequest(1, 16), KVRequest(2, 16)))
+    a = eng.acquire()
+    eng.step([(a, [1] * 100)], [[]])
+    before = (eng.cache.free_pages(), eng.cache.slots.num_free, list(eng.cache.groups[0].pages.table(a)))
+
+    class Fails:
+        is_cuda = False
+
+        def __getitem__(self, at):
+            raise RuntimeError("out of memory")
+
+    for group in eng.cache.groups:                      # in the first group, and in the second when the first has been copied
+        with monkeypatch.context() as m:
+            m.setattr(group, "storage", Fails())
+            with pytest.raises(RuntimeError, match="out of memory"):
+                eng.fork(a, 2)
+        assert (eng.cache.free_pages(), eng.cache.slots.num_free, eng.cache.groups[0].pages.table(a)) == before
+    b, = eng.fork(a, 1)
+    eng.release(a)
+    eng.release(b)
+    assert eng.cache.free_pages() == [40, 40] and eng.cache.slots.num_held == 0
