@@ -202,7 +202,7 @@ def run(argv: Optional[List[str]] = None) -> int:
     def generate(prompts: List[List[int]]) -> None:
         print("\n--- Generation ---")
         start = time.perf_counter()
-        if opts.samples > 1:                  # several samples of each prompt, which is run once
+        if opts.samples != 1:                 # several samples of each prompt, which is run once; numbers below one are refused there
             responses = []
             for p in prompts:
                 responses += engine.generate_samples(p, opts.samples, opts.to_sampler_config(), max_tokens=opts.max_tokens,

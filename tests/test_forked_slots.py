@@ -236,3 +236,12 @@ def test_a_fork_whose_copies_fail_leaves_nothing_held(monkeypatch):
     eng.release(a)
     eng.release(b)
     assert eng.cache.free_pages() == [40, 40] and eng.cache.slots.num_held == 0
+
+
+@pytest.mark.parametrize("samples", [0, -3])
+def test_the_command_line_refuses_numbers_of_samples_below_one(monkeypatch, samples):
+    from llmplayer_b200 import cli, engine
+    from llmplayer_b200.errors import RequestError
+    monkeypatch.setattr(engine.Engine, "load", classmethod(lambda cls, *args, **kwargs: engine_on_the_host()))
+    with pytest.raises(RequestError, match="samples"):
+        cli.run(["some_model", "--prompt", "1 2 3", "--samples", str(samples)])
