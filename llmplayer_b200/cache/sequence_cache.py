@@ -268,12 +268,10 @@ class SequenceCache:
         except KeyError:
             raise CacheError(f"slot {slot} is not held") from None
 
-    def births(self, slots: Sequence[int]) -> List[int]:
-        """A number per slot that no sequence before it had: a slot that was released and handed out again has another one, though a fork
-        may have given it the same length at once."""
-        for slot in slots:
-            self.length(slot)
-        return [self._birth[slot] for slot in slots]
+    def births(self, slots: Sequence[int]) -> List[Optional[int]]:
+        """A number per slot that no sequence before it had (None: not held): a slot that was released and handed out again has another
+        one, though a fork may have given it the same length at once."""
+        return list(map(self._birth.get, slots))
 
     def view(self, run: int):
         return self._views[run]

@@ -186,7 +186,9 @@ class Engine:
                 if not ops.attention_shared_pays(ctx.num_sequences, n, ctx.max_new, own, *heads):
                     n = 0
                 elif single:
-                    ctx.shared_until = min(ctx.shared_until, PAGE_SIZE * (n + ops.attention_shared_reach(ctx.num_sequences, n, *heads) // 1))
+                    reach = ops.attention_shared_reach(ctx.num_sequences, n, *heads)
+                    if reach < float("inf"):
+                        ctx.shared_until = min(ctx.shared_until, PAGE_SIZE * (n + int(reach)))
             out.append(n if reads else 0)
         return out
 

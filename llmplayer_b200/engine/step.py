@@ -153,7 +153,7 @@ class StepContext:
         self.workspace = workspace
         self._sequences: Optional[List[SequenceStep]] = sequences
         self.slot_list = [s.slot for s in sequences]
-        self.births: Optional[List[int]] = None        # set by the engine: which sequences the slots held when this was described
+        self.births: Optional[List[Optional[int]]] = None        # set by the engine: which sequences the slots held when this was described
         self.first_positions = [s.first_position for s in sequences]
         self.new_counts = [s.num_new for s in sequences]
         self.num_tokens = T = len(tokens)
