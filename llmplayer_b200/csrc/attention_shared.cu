@@ -12,11 +12,11 @@
 //                  begin before the first kernel's results are there (programmatic launch), as far as the SMs have room. Few rows of
 //                  several tokens have many results, which a third kernel joins.
 //
-// B200, 32 query heads on 8, caches cold, the whole call in a graph, against attention that reads every sequence's pages:
-//   64 single tokens, heads of 128, 128 shared pages, up to 250 own positions each: 37 us against 432; the two kernels by
+// B200, 32 query heads on 8, calls one behind the other in a graph, each on a cache that has left L2, against attention that reads every sequence's pages:
+//   64 single tokens, heads of 128, 128 shared pages, up to 250 own positions each: 26.7 us against 427; the two kernels by
 //       themselves 21 and 15 us for 70 MB (10.8 us at the measured copy rate).
-//   24 sequences of 9 to 37 tokens, heads of 64, 50 shared pages: 43 against 231; 33 and 12 us for 15 GFLOP.
-//   40 sequences of 47 to 190 tokens, heads of 128, 500 shared pages: 1,890 against 5,380, 1,298 TFLOP/s, 80 % of the measured rate of
+//   24 sequences of 9 to 37 tokens, heads of 64, 50 shared pages: 33.8 against 223; 33 and 12 us, by themselves and cold, for 15 GFLOP.
+//   40 sequences of 47 to 190 tokens, heads of 128, 500 shared pages: 1,890 against 5,500, 1,298 TFLOP/s, 80 % of the measured rate of
 //       dense products (96 us of it the second kernel); 2,100 over a long run, where the power limit holds the clock down.
 //
 // All sums, maxima and partial results are float32. The softmax weights enter the products with the values as bfloat16, rounded
