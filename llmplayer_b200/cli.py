@@ -189,6 +189,7 @@ def run(argv: Optional[List[str]] = None) -> int:
         from .weights import write_random_model
         write_random_model(load_config(opts.model_path), opts.random_seed, opts.model_path, dtype=opts.dtype)
     from .engine import Engine
+    from .engine.generate import GenerationStats
     prompts = [parse_ids(p) for p in opts.prompts]
     if opts.prompt_file is not None:
         with open(opts.prompt_file) as fh:
@@ -203,21 +204,23 @@ def run(argv: Optional[List[str]] = None) -> int:
         print("\n--- Generation ---")
         start = time.perf_counter()
         if opts.samples != 1:                 # several samples of each prompt, which is run once; numbers below one are refused there
-            responses = []
+            responses, stats = [], []
             for p in prompts:
                 responses += engine.generate_samples(p, opts.samples, opts.to_sampler_config(), max_tokens=opts.max_tokens,
                                                      stop_token_ids=opts.stop_ids, logprobs=opts.logprobs)
+                stats.append(engine.last_generation_stats)
         else:
             responses = engine.generate(prompts, opts.to_sampler_config(), max_tokens=opts.max_tokens,
                                         stop_token_ids=opts.stop_ids, logprobs=opts.logprobs)
+            stats = [engine.last_generation_stats]
         elapsed_ms = (time.perf_counter() - start) * 1e3
         for i, r in enumerate(responses):
             _print_result(i, len(responses), r)
-        stats = engine.last_generation_stats
+        total = GenerationStats(generated_tokens=sum(s.generated_tokens for s in stats), decode_ms=sum(s.decode_ms for s in stats))
         print("--- Stats ---")
         print("Tokens: %d prompt + %d generated in %dms (%.1f tok/s)" % (
-            sum(r.prompt_token_count for r in responses), sum(r.token_count for r in responses),
-            elapsed_ms, stats.decode_tokens_per_second))
+            sum(len(p) for p in prompts), sum(r.token_count for r in responses),
+            elapsed_ms, total.decode_tokens_per_second))
         if opts.profile:
             # as the reference's -Dcuda.profile=true prints: milliseconds per section (java21
             # inference/CudaForwardPass.java:1431-1456)

@@ -245,3 +245,27 @@ def test_the_command_line_refuses_numbers_of_samples_below_one(monkeypatch, samp
     monkeypatch.setattr(engine.Engine, "load", classmethod(lambda cls, *args, **kwargs: engine_on_the_host()))
     with pytest.raises(RequestError, match="samples"):
         cli.run(["some_model", "--prompt", "1 2 3", "--samples", str(samples)])
+
+
+def test_the_command_line_counts_a_prompt_once_and_all_prompts_samples(monkeypatch, capsys):
+    from llmplayer_b200 import cli, engine
+    from llmplayer_b200.engine.generate import GenerationResponse, GenerationStats
+
+    class Counting:
+        def generate_samples(self, prompt, samples, *args, **kwargs):
+            # 10 tokens of each sample at 100 or 300 tokens a second
+            ms = samples * 10 / (100 if prompt == [1, 2, 3] else 300) * 1e3
+            self.last_generation_stats = GenerationStats(generated_tokens=10 * samples, decode_ms=ms)
+            return [GenerationResponse([5] * 10, len(prompt), "length") for _ in range(samples)]
+
+        def generate(self, prompts, *args, **kwargs):
+            self.last_generation_stats = GenerationStats(generated_tokens=10 * len(prompts), decode_ms=200.0)
+            return [GenerationResponse([5] * 10, len(p), "length") for p in prompts]
+
+    monkeypatch.setattr(engine.Engine, "load", classmethod(lambda cls, *args, **kwargs: Counting()))
+    cli.run(["some_model", "--prompt", "1 2 3", "--prompt", "4 5", "--samples", "3"])
+    out = capsys.readouterr().out
+    assert "Tokens: 5 prompt + 60 generated" in out and "(150.0 tok/s)" in out
+    cli.run(["some_model", "--prompt", "1 2 3", "--prompt", "4 5"])
+    out = capsys.readouterr().out
+    assert "Tokens: 5 prompt + 20 generated" in out and "(100.0 tok/s)" in out
