@@ -106,7 +106,7 @@ class Model:
         out = [False] * len(cache.groups)
 
         def look(mixer, view) -> None:
-            if isinstance(view, BundleView):
+            if isinstance(view, BundleView) and hasattr(mixer, "children"):
                 for member, members_view in zip(mixer.children(), view.members):
                     look(member, members_view)
             elif isinstance(view, KVView) and hasattr(mixer, "reads_shared_pages") and mixer.reads_shared_pages(view):

@@ -1315,16 +1315,16 @@ def attention_shared_serves(num_heads: int, num_kv_heads: int, head_dim: int, pa
 # Single tokens. The other form rotates, stores and attends in one kernel, and shares a sequence's own pages out over the SMs, where here one CTA goes
 # through them one behind the other: 0.74 us (heads of 64) or 0.89 (128) per page from the fifth on, unless the batch is large enough for its reads to take
 # longer. That and 8 us are set against 0.032 ns for each page, key/value head and feature that is not read again; counted in 64 features, 2 ns:
-#   8 sequences on 128 pages, 4 own pages 59 / 96 us against 61 / 118; 64 own pages 94 / 165 against 70 / 153; 200 own pages 199 / 297 against 90 / 190
-#   64 on 8, 16 own 94 / 168 against 90 / 190; 16 on 32, 4 own 58 / 113 against 57 / 123; 2 on 512, 4 own 71 / 131 against 61 / 139; 200 own 198 / 300 against 68 / 151
+#   8 sequences on 128 pages, 4 own pages 59 / 114 us against 61 / 136; 64 own pages 94 / 165 against 70 / 153; 200 own pages 199 / 297 against 90 / 190
+#   64 on 16, 16 own 94 / 168 against 90 / 190; 16 on 32, 4 own 58 / 113 against 57 / 123; 2 on 512, 4 own 71 / 131 against 61 / 139; 200 own 198 / 300 against 68 / 151
 SHARED_PAGES_SINGLE = 3900
 # Several tokens, runs of up to 64: the other form goes through all pages of a sequence one behind the other as well, so shared ones alone are counted:
-#   24 tokens each, none of their own before: 2 sequences on 8 pages 59 / 117 against 64 / 128; 8 on 4 107 / 212 against 103 / 209, on 8 106 / 212 against 109 / 219;
+#   24 tokens each, none of their own before: 2 sequences on 8 pages 59 / 117 against 64 / 128; 8 on 4 107 / 212 against 103 / 209, on 8 106 / 213 against 109 / 219;
 #   60 on 1 209 / 606 against 242 / 648
-# Longer runs have tcgen05 there, and mma.sync here for the own pages; the shared ones run at 1.3 to 2.5 times the other form's rate. Both go with the tokens, so
+# Longer runs have tcgen05 there, and mma.sync here for the own pages; the shared ones run at 1.3 to 2.9 times the other form's rate. Both go with the tokens, so
 # what counts are a token's keys: its own ones twice, and 1,200 for the results' way, against the shared ones.
-#   8 sequences of 400 tokens on 4 pages 418 / 1,229 against 411 / 1,156, on 64 544 / 1,350 against 601 / 1,506; with 100 own pages on 64 1,071 / 2,334 against 943 / 2,188
-#   and on 256 1,482 / 2,741 against 1,601 / 3,378; 60 of 96 on 4 669 / 2,210 against 666 / 2,012, on 64 883 / 2,381 against 1,011 / 2,681
+#   8 sequences of 400 tokens on 8 pages 418 / 1,229 against 411 / 1,156, on 64 544 / 1,350 against 601 / 1,506; with 100 own pages on 64 1,071 / 2,334 against 943 / 2,188
+#   and on 256 1,482 / 2,741 against 1,601 / 3,378; 60 of 96 on 8 669 / 2,210 against 666 / 2,012, on 64 883 / 2,381 against 1,011 / 2,681
 SHARED_PAGES_SEVERAL = 40
 
 

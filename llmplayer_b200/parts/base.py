@@ -8,7 +8,9 @@ step. No part knows which model it is in.
 * Position:      owned by a mixer: ``rotation()`` (a rule the kernels apply on the way) or
                  ``apply(ctx, qkv, ...)`` (any other rule, applied to the projection in place)
 * Mixer:         ``cache_request()`` and ``forward(ctx, cache_view, x[T, d], residual[T, d])``:
-                 adds its output into the float32 residual stream
+                 adds its output into the float32 residual stream. One that attends over a page group may say
+                 ``reads_shared_pages(cache_view)``: that it attends over the first ``ctx.shared_pages`` pages of the
+                 group, which all of a step's sequences begin with, once for all of them
 * Feed-forward:  ``forward(ctx, x[T, d], residual[T, d])``: adds into the residual stream
 * Block:         ``forward(ctx, cache_view, residual[T, d])``: one layer, in place
 
@@ -126,7 +128,7 @@ class Part:
     # Steps of one token per sequence are replayed from CUDA graphs that were captured on an earlier step of
     # the same shape, possibly for other sequences. A part whose ``forward`` depends on the step only through
     # the device tensors of ``ctx`` (``tokens``, ``positions``, ``slots``, ``kv_len``, ``page_tables``...) and
-    # through what the graph's key holds (batch, page-table widths, wanted rows) may say so; a part that reads
+    # through what the graph's key holds (batch, page-table widths, ``shared_pages``, wanted rows) may say so; a part that reads
     # the step on the host (``ctx.sequences``, ``ctx.slot_list``: which rows of a state it updates, say)
     # leaves this False, and a model with such a part runs every step directly.
     capture_safe = False

@@ -9,10 +9,10 @@ from test_forked_slots import engine_on_the_host, step
 MEASURED = [
     (64, 8, 128, 4, 1, 61, 59), (64, 8, 128, 64, 1, 70, 94), (64, 8, 128, 200, 1, 90, 199), (64, 2, 512, 4, 1, 61, 71), (64, 2, 512, 200, 1, 68, 198),
     (64, 64, 8, 0, 1, 60, 61), (64, 64, 16, 0, 1, 68, 63), (64, 64, 16, 200, 1, 329, 313), (64, 32, 128, 64, 1, 158, 114), (64, 16, 512, 64, 1, 211, 143),
-    (64, 4, 128, 200, 1, 66, 198), (128, 8, 128, 4, 1, 118, 96), (128, 8, 128, 64, 1, 153, 165), (128, 8, 128, 200, 1, 190, 297), (128, 2, 512, 4, 1, 139, 131),
-    (128, 2, 512, 200, 1, 151, 300), (128, 4, 512, 200, 1, 190, 310), (128, 64, 8, 16, 1, 190, 168), (128, 16, 16, 64, 1, 150, 171), (128, 16, 64, 0, 1, 138, 113),
+    (64, 4, 128, 200, 1, 66, 198), (128, 8, 128, 4, 1, 136, 114), (128, 8, 128, 64, 1, 153, 165), (128, 8, 128, 200, 1, 190, 297), (128, 2, 512, 4, 1, 139, 131),
+    (128, 2, 512, 200, 1, 151, 300), (128, 4, 512, 200, 1, 190, 310), (128, 64, 16, 16, 1, 190, 168), (128, 16, 16, 64, 1, 150, 171), (128, 16, 64, 0, 1, 138, 113),
     (64, 2, 16, 0, 24, 76, 61), (64, 8, 4, 0, 24, 103, 107), (128, 8, 4, 0, 24, 209, 212), (64, 60, 1, 0, 24, 242, 209), (128, 20, 64, 100, 24, 1386, 620),
-    (64, 4, 8, 100, 1600, 1392, 1925), (128, 4, 16, 100, 96, 401, 584), (128, 2, 64, 100, 96, 341, 493), (128, 60, 4, 0, 96, 2012, 2210), (64, 60, 4, 0, 96, 666, 669),
+    (64, 4, 8, 100, 1600, 1392, 1925), (128, 4, 16, 100, 96, 401, 584), (128, 2, 64, 100, 96, 341, 493), (128, 60, 8, 0, 96, 2012, 2210), (64, 60, 8, 0, 96, 666, 669),
     (64, 60, 64, 0, 96, 1011, 883), (64, 8, 64, 0, 400, 601, 544), (64, 8, 64, 100, 400, 943, 1071), (64, 8, 256, 100, 400, 1601, 1482), (128, 8, 256, 100, 400, 3378, 2741),
     (128, 2, 256, 16, 1600, 2617, 2016), (64, 20, 256, 0, 96, 873, 584)]
 
@@ -128,3 +128,24 @@ def test_a_decode_goes_on_over_the_end_of_a_choice(tmp_path, monkeypatch, way):
         compare("a choice of shared pages, over its end")
     assert eng._last_ctx.shared_pages == [0] and max(map(len, told)) > until
     eng.check()
+
+
+@pytest.mark.gpu
+def test_which_groups_can_be_attended_over_once(tmp_path):
+    """The bfloat16 form of a plain design; not float32, and not what the kernel is not built for (scores with windows, caps or biases; states)."""
+    import dopuvik_helpers
+    import ramupel_helpers
+    from helpers import make_model
+    from llmplayer_b200 import Engine
+
+    def groups(eng):
+        found = eng.model.groups_sharing_pages(eng.cache)
+        assert len(found) == len(eng.cache.groups)
+        return found
+
+    assert groups(Engine.load(make_model(tmp_path / "a", "D"), context_length=128, max_batch=2)) == [True]
+    assert groups(Engine.load(make_model(tmp_path / "b", "D", dtype="float32"), dtype="float32", context_length=128, max_batch=2)) == [False]
+    for kit, name in ((ramupel_helpers, "small"), (dopuvik_helpers, sorted(dopuvik_helpers.CONFIGS)[0])):
+        eng = Engine.load(kit.make_model(tmp_path, name, "bfloat16"), max_tokens=512, max_slots=2)
+        for found, group in zip(groups(eng), eng.cache.groups):
+            assert not found or (group.request.window is None and group.request.head_dim in (64, 128))
